@@ -15,6 +15,9 @@
  * code (the reference's entry points return void), a batched variant, and a
  * stream-ordered device-pointer API for callers that keep activations in HBM.
  *
+ * Part 3 is additive too: an 8-bit paged KV cache with its attention and page
+ * operators, and token log probabilities.
+ *
  * Numerics: every output is bit-identical to the reference's scalar build of
  * src/quant.c (quantized activations, int32 unit sums and fp32 outputs), with
  * one documented exception: for Q4_K the reference's vec_dot_q4K_q8_0
@@ -56,10 +59,12 @@ typedef struct {
 
 /* GGML type ids accepted as `type` (reference include/gguf.h:28-42). */
 #define QUANTR_TYPE_F32  0u
+#define QUANTR_TYPE_F16  1u  /* activations and logits of the serving operators (Part 3) only */
 #define QUANTR_TYPE_Q8_0 8u
 #define QUANTR_TYPE_Q4_K 12u
 #define QUANTR_TYPE_Q5_K 13u
 #define QUANTR_TYPE_Q6_K 14u
+#define QUANTR_TYPE_BF16 30u /* as QUANTR_TYPE_F16 */
 
 /* ---------------------------------------------------------------------------
  * Part 1: reference-compatible entry points (host pointers, synchronous).
@@ -106,7 +111,8 @@ enum {
     QUANTR_ERR_TOO_LARGE = 7,        /* shape exceeds a kernel limit */
     QUANTR_ERR_WORKSPACE = 8,        /* caller workspace too small */
     QUANTR_ERR_ROUTING = 9,          /* a token's router probabilities were not finite */
-    QUANTR_ERR_UNREGISTERED = 10     /* host weights not covered by quantr_gpu_register_weights */
+    QUANTR_ERR_UNREGISTERED = 10,    /* host weights not covered by quantr_gpu_register_weights */
+    QUANTR_ERR_PAGES = 11            /* a cache page was missing, outside the pool, or none was left */
 };
 int quantr_gpu_last_error(void);
 void quantr_gpu_clear_error(void);
@@ -464,6 +470,146 @@ int quantr_debug_expf_dev(float* out, uint32_t first, long long n, void* stream)
 #define QUANTR_NOALLOC_SCRATCH_BYTES (1u << 20)
 int quantr_gemv_noalloc_dev(float* out, long long ldo, const float* x, long long ldx, const void* w,
                             uint32_t type, int n, int d, int B, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Part 3: serving several continuations - an 8-bit paged KV cache, attention
+ * over it, its page operators, and token log probabilities.  No counterpart in
+ * the reference, whose KV cache is one fp32 or fp16 array (src/model.c:128-137,
+ * src/runtime.c:74-92) and whose samplers see one token's logits.
+ *
+ * All pointers inside the structs and arguments are device pointers, except the
+ * structs themselves, which the host reads during the call.  Every call is
+ * asynchronous on `stream`, allocates nothing and can be captured (the first
+ * call on a device allocates its error word: make it before any capture).
+ * What only the device can see - a slot or page id out of range, a table too
+ * short for a length, an empty pool - is skipped as each call describes and
+ * reported by quantr_gpu_device_status as QUANTR_ERR_PAGES.
+ * -------------------------------------------------------------------------*/
+
+/* Pool of cache pages.  A page holds page_tokens tokens of every layer and KV
+ * head; an element is an 8-bit code times the scale of its (page, layer, head):
+ *   code  of token t, element i: k[(((page*n_layers + layer)*n_kv_heads + head)*page_tokens + t)*head_dim + i]
+ *   scale: k_scale[(page*n_layers + layer)*n_kv_heads + head]
+ * and the same for v.  page_tokens is 32, 64 or 128; head_dim a multiple of 16
+ * up to 128; k and v are 16-byte aligned; n_pages*n_layers*n_kv_heads < 2^31. */
+typedef struct {
+    int8_t* k;
+    int8_t* v;
+    float* k_scale;
+    float* v_scale;
+    int n_pages, n_layers, n_kv_heads, page_tokens, head_dim;
+} quantr_kv8_pool;
+
+/* Page tables of `slots` sequences: token t of the sequence in slot s is token
+ * t % page_tokens of page table[s*max_pages + t/page_tokens]; entries at or
+ * past ceil(lens[s]/page_tokens) are -1.  refs[page] (n_pages of them) counts
+ * the table entries that name the page; 0 = free.  An empty set of tables is
+ * table = -1, lens = 0, refs = 0. */
+typedef struct {
+    int* table;
+    int* lens;
+    int* refs;
+    int slots, max_pages;
+} quantr_kv8_tables;
+
+/* A ragged batch of rows (new tokens, query tokens): sequence b of B is slot
+ * slot[b] (NULL: b) and has the rows start[b] .. start[b+1]-1 (NULL start:
+ * max_rows rows each), at most max_rows of them.  Its rows are the LAST tokens
+ * of the sequence: with n rows, row i stands at position lens - n + i, so lens
+ * already counts them (quantr_kv8_extend_dev).  No slot appears twice. */
+typedef struct {
+    const int* slot;
+    const int* start;
+    int B, max_rows;
+} quantr_kv8_batch;
+
+/* Writes the rows' keys and values (element i of head h of row r at
+ * k[r*ldk + h*head_dim + i], type F32/F16/BF16) into layer `layer`.  A page
+ * whose first token is among the rows gets, per head, the scale
+ * max(max|x|/127, 2^-126); a page that already held tokens keeps its scale s,
+ * doubled until 127*s covers the new rows, its old codes being rounded again
+ * (half to even).  Doubling bounds what repeated rounding adds: at most one
+ * step of the final scale, however many rows a page gets one by one.
+ * code = clamp(rint(x * (1/s)), -127, 127) in fp32.  A row element that is not
+ * finite makes the scale NaN: attention to that page then answers NaN instead
+ * of a plausible number, until the page is begun anew.  Rows whose position or
+ * page does not exist are skipped. */
+int quantr_kv8_append_dev(const void* k, long long ldk, const void* v, long long ldv, uint32_t type,
+                          const quantr_kv8_pool* pool, const quantr_kv8_tables* tables,
+                          const quantr_kv8_batch* batch, int layer, void* stream);
+
+/* The inverse: the rows' keys and values as code*scale, rounded once to
+ * `type`.  Rows that do not exist read as zeros. */
+int quantr_kv8_read_dev(void* k, long long ldk, void* v, long long ldv, uint32_t type, const quantr_kv8_pool* pool,
+                        const quantr_kv8_tables* tables, const quantr_kv8_batch* batch, int layer, void* stream);
+
+/* Attention of the rows over the cache.  Row r at position p, query head h
+ * (q[r*ldq + h*head_dim + i], KV head h / (n_heads/n_kv_heads)):
+ *   x_t = scale * q . k_t for max(0, p-window+1) <= t <= p (window 0: from 0)
+ *   out[r*ldo + h*head_dim + i] = sum_t softmax_t(x) v_t[i]
+ *   lse[r*n_heads + h] = ln sum_t exp(x_t)                    (optional)
+ * q and out have `type` (F32/F16/BF16).  A row that sees nothing (position
+ * below 0, all of its pages missing) gives out = 0, lse = -inf; a page that is
+ * missing counts as masked.  A query or a scale that is not finite gives NaN.
+ * max_len is the longest sequence expected: it sizes the split of long
+ * sequences over the GPU and the workspace; longer ones are right, only
+ * slower.  The workspace must be 256-byte aligned. */
+size_t quantr_kv8_attend_workspace_bytes(const quantr_kv8_pool* pool, const quantr_kv8_batch* batch, int n_heads,
+                                         int max_len);
+int quantr_kv8_attend_dev(void* out, long long ldo, const void* q, long long ldq, uint32_t type, int n_heads,
+                          const quantr_kv8_pool* pool, const quantr_kv8_tables* tables,
+                          const quantr_kv8_batch* batch, int layer, float scale, int window, int max_len, float* lse,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
+/* Tables from tables: slot s of `to` takes the pages of slot from[s] of `in`
+ * (-1: none, the slot is empty).  One slot named several times is a fork, one
+ * named nowhere is freed, and a permutation reorders beams.  Pages are shared,
+ * not copied; to->refs is counted anew.  `in` and `to` have the same shape and
+ * share no memory (a step in flight may go on reading `in`). */
+int quantr_kv8_select_dev(const quantr_kv8_tables* to, const quantr_kv8_tables* in, const int* from,
+                          const quantr_kv8_pool* pool, void* stream);
+
+/* Makes room for n_new[b] more tokens (NULL: 1) of slot[b] (NULL: b), b < B <=
+ * 1024, in this order: allocates the free pages of lowest index, and gives a
+ * sequence whose last, partly filled page is shared its own copy of it (of
+ * several sequences that share it, the last one in the batch keeps it if
+ * nobody else does); then adds n_new to lens.  grown[b] (optional) = 1, or 0
+ * where the sequence was left as it was: its table is too short, or the pages
+ * ran out (then for every later sequence that needs one too). */
+size_t quantr_kv8_pages_workspace_bytes(const quantr_kv8_pool* pool, const quantr_kv8_tables* tables);
+int quantr_kv8_extend_dev(const quantr_kv8_pool* pool, const quantr_kv8_tables* tables, const int* slot,
+                          const int* n_new, int B, int* grown, void* workspace, size_t workspace_bytes,
+                          void* stream);
+
+/* Moves the pages in use to the front of the pool: with n of them, the i-th
+ * one at or past n goes to the i-th free place before n.  Tables and refs
+ * follow; map[page] (n_pages) = its new place (-1: free), n_live[0] = n, both
+ * optional. */
+int quantr_kv8_compact_dev(const quantr_kv8_pool* pool, const quantr_kv8_tables* tables, int* map, int* n_live,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
+/* Copies the contents of page src[i] to page dst[i], i < n, all layers.  No
+ * page may be both read and written, nor written twice. */
+int quantr_kv8_copy_pages_dev(const quantr_kv8_pool* pool, const int* dst, const int* src, int n, void* stream);
+
+/* Log probabilities of rows of logits (x[r*ldl + v], v < vocab, type
+ * F32/F16/BF16), y = x / temperature:
+ *   lse[r]     = ln sum_v exp(y_v)
+ *   logprob[r] = y[token[r]] - lse[r]; 0 where token[r] is -1 (no token
+ *                given), NaN where it is any other id outside the vocabulary
+ *   entropy[r] = -sum_v p_v ln p_v
+ *   top_id[r*k + i], top_logprob[r*k + i]: the k <= 64 largest logits in
+ *                order, of equal ones the lower id first; -1 and -inf where
+ *                fewer than k are above -inf
+ * Each output may be NULL (token too, with logprob).  Logits of -inf have
+ * probability 0.  A row of nothing else gives lse = -inf, logprob = -inf,
+ * entropy = 0; one with a NaN or +inf gives NaN in all three and in
+ * top_logprob (its top_id are the k largest that are not NaN).  The workspace
+ * must be 256-byte aligned. */
+size_t quantr_logprobs_workspace_bytes(int rows, int vocab, int k);
+int quantr_logprobs_dev(const void* x, long long ldl, uint32_t type, int rows, int vocab, float temperature,
+                        const int* token, float* logprob, float* entropy, float* lse, int k, int* top_id,
+                        float* top_logprob, void* workspace, size_t workspace_bytes, void* stream);
 
 #if defined(__GNUC__)
 #pragma GCC visibility pop

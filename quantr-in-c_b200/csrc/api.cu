@@ -74,6 +74,7 @@ int dev_code(int v)
 {
     if (v == DEV_OK) return QUANTR_OK;
     if (v == DEV_ERR_ROUTING) return QUANTR_ERR_ROUTING;
+    if (v == DEV_ERR_PAGES) return QUANTR_ERR_PAGES;
     return QUANTR_ERR_DEVICE_TIMEOUT;
 }
 
@@ -308,6 +309,8 @@ float vec_dot_host(const void* a, const void* b, int k, uint32_t type)
 
 } // namespace
 
+int qr::status_code(cudaError_t e) { return code_of(e); }
+
 int* qr::device_error_word()
 {
     int dev = 0;
@@ -351,6 +354,7 @@ const char* quantr_gpu_error_string(int code)
     case QUANTR_ERR_WORKSPACE: return "workspace too small";
     case QUANTR_ERR_ROUTING: return "router probabilities not finite for some token";
     case QUANTR_ERR_UNREGISTERED: return "weights not registered with quantr_gpu_register_weights";
+    case QUANTR_ERR_PAGES: return "cache page missing, outside the pool, or none left";
     default: return "unknown error";
     }
 }

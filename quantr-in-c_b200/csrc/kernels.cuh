@@ -25,7 +25,7 @@ size_t actq_bytes(int d, int B);
 ActQ actq_carve(void* ws, int d, int B);
 
 // Device error word written by kernels whose bounded waits give up.
-enum : int { DEV_OK = 0, DEV_ERR_WAIT_TIMEOUT = 1, DEV_ERR_ROUTING = 2 };
+enum : int { DEV_OK = 0, DEV_ERR_WAIT_TIMEOUT = 1, DEV_ERR_ROUTING = 2, DEV_ERR_PAGES = 3 };
 
 struct LaunchCfg {
     cudaStream_t stream = nullptr;
@@ -79,6 +79,9 @@ unsigned long long launch_count();
 // Per-device error word that kernels launched through the device API report
 // bounded-wait timeouts into (allocated on first use; api.cu).
 int* device_error_word();
+
+// QUANTR_* code of a CUDA status (api.cu).
+int status_code(cudaError_t e);
 
 // Error word of the allocation-free GEMV (noalloc.cu) on the current device;
 // reset != 0 clears a recorded error.  DEV_OK if that path never ran here.

@@ -21,6 +21,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libquantr_cuda.so")
 
 F32, Q8_0, Q4_K, Q5_K, Q6_K = 0, 8, 12, 13, 14
+F16, BF16 = 1, 30  # activations and logits of the serving operators
 TYPE_NAMES = {F32: "F32", Q8_0: "Q8_0", Q4_K: "Q4_K", Q5_K: "Q5_K", Q6_K: "Q6_K"}
 BLOCK_BYTES = {Q8_0: 34, Q4_K: 144, Q5_K: 176, Q6_K: 210}
 BLOCK_ELEMS = {Q8_0: 32, Q4_K: 256, Q5_K: 256, Q6_K: 256}
@@ -77,6 +78,17 @@ SIGNATURES = {
     "quantr_decoder_launches": (_i, [_vp, _c.POINTER(_i), _c.POINTER(_i)]),
     "quantr_decoder_kv": (_i, [_vp, _c.POINTER(_vp), _c.POINTER(_vp), _c.POINTER(_sz)]),
     "quantr_moe_shared_dev": (_i, [_vp, _ll, _vp, _ll, _i, _vp, _vp, _u32, _vp, _u32, _vp, _u32, _i, _i, _vp]),
+    "quantr_kv8_append_dev": (_i, [_vp, _ll, _vp, _ll, _u32, _vp, _vp, _vp, _i, _vp]),
+    "quantr_kv8_read_dev": (_i, [_vp, _ll, _vp, _ll, _u32, _vp, _vp, _vp, _i, _vp]),
+    "quantr_kv8_attend_workspace_bytes": (_sz, [_vp, _vp, _i, _i]),
+    "quantr_kv8_attend_dev": (_i, [_vp, _ll, _vp, _ll, _u32, _i, _vp, _vp, _vp, _i, _f, _i, _i, _vp, _vp, _sz, _vp]),
+    "quantr_kv8_select_dev": (_i, [_vp, _vp, _vp, _vp, _vp]),
+    "quantr_kv8_pages_workspace_bytes": (_sz, [_vp, _vp]),
+    "quantr_kv8_extend_dev": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _vp, _sz, _vp]),
+    "quantr_kv8_compact_dev": (_i, [_vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "quantr_kv8_copy_pages_dev": (_i, [_vp, _vp, _vp, _i, _vp]),
+    "quantr_logprobs_workspace_bytes": (_sz, [_i, _i, _i]),
+    "quantr_logprobs_dev": (_i, [_vp, _ll, _u32, _i, _i, _f, _vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _sz, _vp]),
 }
 
 
@@ -347,6 +359,106 @@ def moe_layer(xb, E, k, w1, t1, w3, t3, w2, t2, dim, hidden, router=None, logits
 
 def device_status(stream=0, reset=True):
     return int(lib().quantr_gpu_device_status(stream or None, 1 if reset else 0))
+
+
+# --------------------------------------- paged 8-bit KV cache, log probs --
+
+class Kv8Pool(ctypes.Structure):
+    """quantr_kv8_pool (include/quantr_cuda.h)."""
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("n_pages", _i), ("n_layers", _i),
+                ("n_kv_heads", _i), ("page_tokens", _i), ("head_dim", _i)]
+
+    @classmethod
+    def of(cls, k, v, k_scale, v_scale):
+        """The pool of contiguous device tensors: codes of shape (pages, layers,
+        KV heads, page tokens, head dim), scales (pages, layers, KV heads)."""
+        return cls(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), *k.shape)
+
+
+class Kv8Tables(ctypes.Structure):
+    """quantr_kv8_tables (include/quantr_cuda.h)."""
+    _fields_ = [("table", _vp), ("lens", _vp), ("refs", _vp), ("slots", _i), ("max_pages", _i)]
+
+    @classmethod
+    def of(cls, table, lens, refs):
+        """The tables of contiguous int32 device tensors: table (slots, max
+        pages), lens (slots), refs (pages of the pool)."""
+        return cls(table.data_ptr(), lens.data_ptr(), refs.data_ptr(), *table.shape)
+
+
+class Kv8Batch(ctypes.Structure):
+    """quantr_kv8_batch (include/quantr_cuda.h)."""
+    _fields_ = [("slot", _vp), ("start", _vp), ("B", _i), ("max_rows", _i)]
+
+
+def kv8_append_dev(k, ldk, v, ldv, type_, pool, tables, batch, layer, stream=0):
+    rc = lib().quantr_kv8_append_dev(k, ldk, v, ldv, type_, ctypes.byref(pool), ctypes.byref(tables),
+                                     ctypes.byref(batch), layer, stream or None)
+    if rc:
+        raise QuantrError(rc, "quantr_kv8_append_dev")
+
+
+def kv8_read_dev(k, ldk, v, ldv, type_, pool, tables, batch, layer, stream=0):
+    rc = lib().quantr_kv8_read_dev(k, ldk, v, ldv, type_, ctypes.byref(pool), ctypes.byref(tables),
+                                   ctypes.byref(batch), layer, stream or None)
+    if rc:
+        raise QuantrError(rc, "quantr_kv8_read_dev")
+
+
+def kv8_attend_workspace_bytes(pool, batch, n_heads, max_len):
+    return int(lib().quantr_kv8_attend_workspace_bytes(ctypes.byref(pool), ctypes.byref(batch), n_heads, max_len))
+
+
+def kv8_attend_dev(out, ldo, q, ldq, type_, n_heads, pool, tables, batch, layer, scale, max_len, ws, ws_bytes,
+                   window=0, lse=None, stream=0):
+    rc = lib().quantr_kv8_attend_dev(out, ldo, q, ldq, type_, n_heads, ctypes.byref(pool), ctypes.byref(tables),
+                                     ctypes.byref(batch), layer, scale, window, max_len, lse, ws, ws_bytes,
+                                     stream or None)
+    if rc:
+        raise QuantrError(rc, "quantr_kv8_attend_dev")
+
+
+def kv8_select_dev(to, in_, from_, pool, stream=0):
+    """quantr_kv8_select_dev: fork, free or reorder sequences (`to` from `in_`)."""
+    rc = lib().quantr_kv8_select_dev(ctypes.byref(to), ctypes.byref(in_), from_, ctypes.byref(pool), stream or None)
+    if rc:
+        raise QuantrError(rc, "quantr_kv8_select_dev")
+
+
+def kv8_pages_workspace_bytes(pool, tables):
+    return int(lib().quantr_kv8_pages_workspace_bytes(ctypes.byref(pool), ctypes.byref(tables)))
+
+
+def kv8_extend_dev(pool, tables, slot, n_new, B, ws, ws_bytes, grown=None, stream=0):
+    rc = lib().quantr_kv8_extend_dev(ctypes.byref(pool), ctypes.byref(tables), slot, n_new, B, grown, ws, ws_bytes,
+                                     stream or None)
+    if rc:
+        raise QuantrError(rc, "quantr_kv8_extend_dev")
+
+
+def kv8_compact_dev(pool, tables, map_, n_live, ws, ws_bytes, stream=0):
+    rc = lib().quantr_kv8_compact_dev(ctypes.byref(pool), ctypes.byref(tables), map_, n_live, ws, ws_bytes,
+                                      stream or None)
+    if rc:
+        raise QuantrError(rc, "quantr_kv8_compact_dev")
+
+
+def kv8_copy_pages_dev(pool, dst, src, n, stream=0):
+    rc = lib().quantr_kv8_copy_pages_dev(ctypes.byref(pool), dst, src, n, stream or None)
+    if rc:
+        raise QuantrError(rc, "quantr_kv8_copy_pages_dev")
+
+
+def logprobs_workspace_bytes(rows, vocab, k):
+    return int(lib().quantr_logprobs_workspace_bytes(rows, vocab, k))
+
+
+def logprobs_dev(x, ldl, type_, rows, vocab, token, logprob, entropy, k, top_id, top_logprob, ws, ws_bytes,
+                 temperature=1.0, lse=None, stream=0):
+    rc = lib().quantr_logprobs_dev(x, ldl, type_, rows, vocab, temperature, token, logprob, entropy, lse, k, top_id,
+                                   top_logprob, ws, ws_bytes, stream or None)
+    if rc:
+        raise QuantrError(rc, "quantr_logprobs_dev")
 
 
 # --------------------------------------------------------------- decoder --
