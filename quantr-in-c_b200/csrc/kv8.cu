@@ -1,8 +1,8 @@
 // kv8.cu -- the 8-bit paged KV cache: writing rows into pages, reading them
-// back, and attention over them (public contract: include/quantr_cuda.h).
+// back (public contract: include/quantr_cuda.h).
 #include "kv8.cuh"
 
-#include <cmath>
+#include <algorithm>
 
 namespace qr {
 namespace {
@@ -147,107 +147,6 @@ __global__ void __launch_bounds__(kReadThreads) k_kv8_read(const ReadArgs a)
     }
 }
 
-// ----------------------------------------------------------------- attend --
-
-struct AttendArgs {
-    Kv8View w;
-    const void* q;
-    void* out;
-    float* lse;
-    long long ldq, ldo;
-    int H, G, window;
-    float scale;
-};
-
-constexpr int kAttThreads = 128;
-
-// One CTA per (row, query head): tiles of 128 tokens, one running maximum and
-// sum, thread t scores token t and then owns output element t.
-template <typename T>
-__global__ void __launch_bounds__(kAttThreads) k_kv8_attend(const AttendArgs a)
-{
-    __shared__ float qs[128], ps[kAttThreads], red[kAttThreads / 32];
-    pdl_wait();
-    const Kv8View& w = a.w;
-    const int b = blockIdx.x / w.max_rows, i = blockIdx.x % w.max_rows, hq = blockIdx.y, h = hq / a.G;
-    const Kv8Seq s = kv8_seq(w, b);
-    if (i >= s.n) return;
-    const int tid = threadIdx.x, pos = s.len - s.n + i;
-    const size_t row = (size_t)s.row0 + i;
-    bool bad = false;
-    if (tid < w.hd) {
-        qs[tid] = to_f<T>(static_cast<const T*>(a.q)[row * a.ldq + (size_t)hq * w.hd + tid]);
-        bad = !(fabsf(qs[tid]) <= 3.402823466e38f);
-    }
-    bad = __syncthreads_or(bad);
-    float m = -INFINITY, l = 0.0f, o = 0.0f;
-    const int t0 = a.window ? max(pos - a.window + 1, 0) : 0;
-    for (int base = t0 & ~127; base <= pos; base += 128) {
-        const int t = base + tid;
-        float x = -INFINITY;
-        const int unit = t >= t0 && t <= pos ? kv8_unit(w, s, t >> w.lgP, h) : -1;
-        if (unit >= 0) {
-            const int8_t* k = w.k + ((size_t)unit * w.P + (t & (w.P - 1))) * w.hd;
-            float d = 0.0f;
-            for (int e = 0; e < w.hd; ++e) d = fmaf(qs[e], (float)k[e], d);
-            x = d * w.ks[unit] * a.scale;
-        }
-        float mt = x;
-        bool nan = x != x || (bad && unit >= 0);
-        for (int z = 16; z; z >>= 1) mt = fmaxf(mt, __shfl_xor_sync(~0u, mt, z));
-        if ((tid & 31) == 0) red[tid >> 5] = mt;
-        nan = __syncthreads_or(nan);
-        mt = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-        const float mn = nan ? NAN : fmaxf(m, mt);
-        if (mn == -INFINITY) {
-            __syncthreads();
-            continue;
-        }
-        const float f = expf(m - mn), p = unit >= 0 ? expf(x - mn) : 0.0f;
-        ps[tid] = p;
-        float sum = p;
-        __syncthreads();
-        for (int z = 16; z; z >>= 1) sum += __shfl_xor_sync(~0u, sum, z);
-        if ((tid & 31) == 0) red[tid >> 5] = sum;
-        __syncthreads();
-        l = l * f + (red[0] + red[1] + red[2] + red[3]);
-        o *= f;
-        if (tid < w.hd)
-            for (int j = max(t0 - base, 0); j < 128 && base + j <= pos; ++j) {
-                const int u = kv8_unit(w, s, (base + j) >> w.lgP, h);
-                if (u < 0) continue;
-                o = fmaf(ps[j], w.vs[u] * (float)w.v[((size_t)u * w.P + ((base + j) & (w.P - 1))) * w.hd + tid], o);
-            }
-        m = mn;
-        __syncthreads();
-    }
-    if (tid < w.hd)
-        static_cast<T*>(a.out)[row * a.ldo + (size_t)hq * w.hd + tid] = from_f<T>(m == -INFINITY ? 0.0f : o / l);
-    if (a.lse && tid == 0) a.lse[row * a.H + hq] = m == -INFINITY ? -INFINITY : m + logf(l);
-}
-
-int check_rows(const void* p, long long ld, long long need)
-{
-    return p && ld >= need ? QUANTR_OK : QUANTR_ERR_BAD_ARG;
-}
-
-int check_call(const quantr_kv8_pool* pool, const quantr_kv8_tables* tables, const quantr_kv8_batch* batch, int layer,
-               uint32_t type)
-{
-    int rc = kv8_check_pool(pool);
-    if (!rc) rc = kv8_check_tables(tables);
-    if (!rc) rc = kv8_check_batch(batch);
-    if (!rc && (layer < 0 || layer >= pool->n_layers)) rc = QUANTR_ERR_BAD_ARG;
-    if (!rc && !kv8_float_type(type)) rc = QUANTR_ERR_UNSUPPORTED_TYPE;
-    return rc;
-}
-
-int done(cudaError_t e)
-{
-    if (e != cudaSuccess) cudaGetLastError();
-    return status_code(e);
-}
-
 } // namespace
 } // namespace qr
 
@@ -259,10 +158,10 @@ int quantr_kv8_append_dev(const void* k, long long ldk, const void* v, long long
                           const quantr_kv8_pool* pool, const quantr_kv8_tables* tables,
                           const quantr_kv8_batch* batch, int layer, void* stream)
 {
-    int rc = check_call(pool, tables, batch, layer, type);
+    int rc = kv8_check_call(pool, tables, batch, layer, type);
     if (rc || batch->B == 0 || batch->max_rows == 0) return rc;
     const long long need = (long long)pool->n_kv_heads * pool->head_dim;
-    if ((rc = check_rows(k, ldk, need)) || (rc = check_rows(v, ldv, need))) return rc;
+    if ((rc = kv8_check_rows(k, ldk, need)) || (rc = kv8_check_rows(v, ldv, need))) return rc;
     AppendArgs a{};
     a.w = kv8_view(pool, tables, batch, layer);
     const int bytes = type == QUANTR_TYPE_F32 ? 4 : 2;
@@ -272,7 +171,7 @@ int quantr_kv8_append_dev(const void* k, long long ldk, const void* v, long long
     if (span * batch->B > 0x7fffffffll || pool->n_kv_heads > 65535) return QUANTR_ERR_TOO_LARGE;
     LaunchCfg c;
     c.stream = (cudaStream_t)stream;
-    return done(with_type(type, [&](auto* t) {
+    return kv8_done(with_type(type, [&](auto* t) {
         using T = std::remove_const_t<std::remove_pointer_t<decltype(t)>>;
         return launch_ex(k_kv8_append<T>, dim3((unsigned)(span * batch->B), pool->n_kv_heads, 2), kAppendThreads, 0, c, a);
     }));
@@ -281,10 +180,10 @@ int quantr_kv8_append_dev(const void* k, long long ldk, const void* v, long long
 int quantr_kv8_read_dev(void* k, long long ldk, void* v, long long ldv, uint32_t type, const quantr_kv8_pool* pool,
                         const quantr_kv8_tables* tables, const quantr_kv8_batch* batch, int layer, void* stream)
 {
-    int rc = check_call(pool, tables, batch, layer, type);
+    int rc = kv8_check_call(pool, tables, batch, layer, type);
     if (rc || batch->B == 0 || batch->max_rows == 0) return rc;
     const long long need = (long long)pool->n_kv_heads * pool->head_dim;
-    if ((rc = check_rows(k, ldk, need)) || (rc = check_rows(v, ldv, need))) return rc;
+    if ((rc = kv8_check_rows(k, ldk, need)) || (rc = kv8_check_rows(v, ldv, need))) return rc;
     if (batch->B > 65535) return QUANTR_ERR_TOO_LARGE;
     ReadArgs a{};
     a.w = kv8_view(pool, tables, batch, layer);
@@ -294,44 +193,9 @@ int quantr_kv8_read_dev(void* k, long long ldk, void* v, long long ldv, uint32_t
     const long long chunks = ((long long)batch->max_rows * (need / 4) + kReadThreads - 1) / kReadThreads;
     LaunchCfg c;
     c.stream = (cudaStream_t)stream;
-    return done(with_type(type, [&](auto* t) {
+    return kv8_done(with_type(type, [&](auto* t) {
         using T = std::remove_const_t<std::remove_pointer_t<decltype(t)>>;
         return launch_ex(k_kv8_read<T>, dim3((unsigned)std::min(chunks, 4096ll), batch->B, 2), kReadThreads, 0, c, a);
-    }));
-}
-
-size_t quantr_kv8_attend_workspace_bytes(const quantr_kv8_pool* pool, const quantr_kv8_batch* batch, int n_heads,
-                                         int max_len)
-{
-    (void)pool, (void)batch, (void)n_heads, (void)max_len;
-    return 256;
-}
-
-int quantr_kv8_attend_dev(void* out, long long ldo, const void* q, long long ldq, uint32_t type, int n_heads,
-                          const quantr_kv8_pool* pool, const quantr_kv8_tables* tables,
-                          const quantr_kv8_batch* batch, int layer, float scale, int window, int max_len, float* lse,
-                          void* workspace, size_t workspace_bytes, void* stream)
-{
-    int rc = check_call(pool, tables, batch, layer, type);
-    if (rc) return rc;
-    if (n_heads <= 0 || n_heads % pool->n_kv_heads || window < 0 || max_len < 0 || !std::isfinite(scale))
-        return QUANTR_ERR_BAD_ARG;
-    if (batch->B == 0 || batch->max_rows == 0) return QUANTR_OK;
-    const long long need = (long long)n_heads * pool->head_dim;
-    if ((rc = check_rows(out, ldo, need)) || (rc = check_rows(q, ldq, need))) return rc;
-    if ((long long)batch->B * batch->max_rows > 0x7fffffffll || n_heads > 65535) return QUANTR_ERR_TOO_LARGE;
-    if (!workspace || ((uintptr_t)workspace & 255) ||
-        workspace_bytes < quantr_kv8_attend_workspace_bytes(pool, batch, n_heads, max_len))
-        return QUANTR_ERR_WORKSPACE;
-    AttendArgs a{};
-    a.w = kv8_view(pool, tables, batch, layer);
-    a.q = q, a.out = out, a.lse = lse, a.ldq = ldq, a.ldo = ldo;
-    a.H = n_heads, a.G = n_heads / pool->n_kv_heads, a.window = window, a.scale = scale;
-    LaunchCfg c;
-    c.stream = (cudaStream_t)stream;
-    return done(with_type(type, [&](auto* t) {
-        using T = std::remove_const_t<std::remove_pointer_t<decltype(t)>>;
-        return launch_ex(k_kv8_attend<T>, dim3(batch->B * batch->max_rows, n_heads), kAttThreads, 0, c, a);
     }));
 }
 

@@ -41,6 +41,28 @@ inline int kv8_check_batch(const quantr_kv8_batch* b)
     return b && b->B >= 0 && b->max_rows >= 0 ? QUANTR_OK : QUANTR_ERR_BAD_ARG;
 }
 
+inline int kv8_check_rows(const void* p, long long ld, long long need)
+{
+    return p && ld >= need ? QUANTR_OK : QUANTR_ERR_BAD_ARG;
+}
+
+inline int kv8_check_call(const quantr_kv8_pool* pool, const quantr_kv8_tables* tables, const quantr_kv8_batch* batch, int layer,
+               uint32_t type)
+{
+    int rc = kv8_check_pool(pool);
+    if (!rc) rc = kv8_check_tables(tables);
+    if (!rc) rc = kv8_check_batch(batch);
+    if (!rc && (layer < 0 || layer >= pool->n_layers)) rc = QUANTR_ERR_BAD_ARG;
+    if (!rc && !kv8_float_type(type)) rc = QUANTR_ERR_UNSUPPORTED_TYPE;
+    return rc;
+}
+
+inline int kv8_done(cudaError_t e)
+{
+    if (e != cudaSuccess) cudaGetLastError();
+    return status_code(e);
+}
+
 // The cache as kernels see it: one layer's scales and codes are reached by the
 // unit (page*n_layers + layer)*n_kv_heads + head, a 31-bit number; byte offsets
 // are 64-bit.

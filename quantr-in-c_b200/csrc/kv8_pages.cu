@@ -284,12 +284,6 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv8_compact(const PlanArgs a)
     }
 }
 
-int done(cudaError_t e)
-{
-    if (e != cudaSuccess) cudaGetLastError();
-    return status_code(e);
-}
-
 int lg_tokens(const quantr_kv8_pool* p) { return p->page_tokens == 32 ? 5 : p->page_tokens == 64 ? 6 : 7; }
 
 int copy_grid(long long pages)
@@ -332,7 +326,7 @@ int quantr_kv8_select_dev(const quantr_kv8_tables* to, const quantr_kv8_tables* 
     cudaError_t e = launch_ex(k_kv8_zero, dim3(std::min((pool->n_pages + 255) / 256, 256)), 256, 0, c, to->refs,
                               pool->n_pages);
     if (e == cudaSuccess) e = launch_ex(k_kv8_select, dim3(to->slots), 128, 0, c, a);
-    return done(e);
+    return kv8_done(e);
 }
 
 size_t quantr_kv8_pages_workspace_bytes(const quantr_kv8_pool* pool, const quantr_kv8_tables* tables)
@@ -377,7 +371,7 @@ int quantr_kv8_extend_dev(const quantr_kv8_pool* pool, const quantr_kv8_tables* 
     cudaError_t e = launch_ex(k_kv8_extend, dim3(1), kPlanThreads, 0, c, a);
     CopyArgs k{*pool, a.count, 0, a.src, a.dst, a.err, nullptr, nullptr, 0};
     if (e == cudaSuccess) e = launch_ex(k_kv8_copy, dim3(copy_grid(B)), kCopyThreads, 0, c, k);
-    return done(e);
+    return kv8_done(e);
 }
 
 int quantr_kv8_compact_dev(const quantr_kv8_pool* pool, const quantr_kv8_tables* tables, int* map, int* n_live,
@@ -392,7 +386,7 @@ int quantr_kv8_compact_dev(const quantr_kv8_pool* pool, const quantr_kv8_tables*
     cudaError_t e = launch_ex(k_kv8_compact, dim3(1), kPlanThreads, 0, c, a);
     CopyArgs k{*pool, a.count, 0, a.src, a.dst, a.err, tables->table, a.list, (size_t)tables->slots * tables->max_pages};
     if (e == cudaSuccess) e = launch_ex(k_kv8_copy, dim3(copy_grid(pool->n_pages)), kCopyThreads, 0, c, k);
-    return done(e);
+    return kv8_done(e);
 }
 
 int quantr_kv8_copy_pages_dev(const quantr_kv8_pool* pool, const int* dst, const int* src, int n, void* stream)
@@ -403,7 +397,7 @@ int quantr_kv8_copy_pages_dev(const quantr_kv8_pool* pool, const int* dst, const
     CopyArgs k{*pool, nullptr, n, src, dst, device_error_word(), nullptr, nullptr, 0};
     LaunchCfg c;
     c.stream = (cudaStream_t)stream;
-    return done(launch_ex(k_kv8_copy, dim3(copy_grid(n)), kCopyThreads, 0, c, k));
+    return kv8_done(launch_ex(k_kv8_copy, dim3(copy_grid(n)), kCopyThreads, 0, c, k));
 }
 
 } // extern "C"

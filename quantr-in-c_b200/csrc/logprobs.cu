@@ -138,8 +138,7 @@ int quantr_logprobs_dev(const void* x, long long ldl, uint32_t type, int rows, i
         using T = std::remove_const_t<std::remove_pointer_t<decltype(t)>>;
         return launch_ex(k_logprobs<T>, dim3(rows), kLpThreads, 0, c, a);
     });
-    if (e != cudaSuccess) cudaGetLastError();
-    return status_code(e);
+    return kv8_done(e);
 }
 
 } // extern "C"
