@@ -7,12 +7,14 @@
 //   lse = m/temperature + ln s,  entropy = ln2 (log2 s - e/s).
 // One pass: each logit is read once, whatever is asked for.
 //
-// Alternatives ride on the maximum that the softmax needs anyway: a thread
-// looks at its single elements only when the maximum of its 16 or 32 reaches
-// the threshold, the k-th best key so far.  Keys are (logit, ~id) in 64 bits, all
-// different, so ties go to the lower id and the answer does not depend on the
-// order of the threads.  The first threshold is the k-th best of the threads'
-// maxima, which k different elements reach.
+// Alternatives cost the pass nothing but a store: a thread keeps the maximum of
+// each group of its elements, which the softmax needs anyway.  Then a threshold
+// that k elements reach at least (each warp's ceil(k/8)-th largest thread
+// maximum, the least of the 8 warps), and only the groups that reach it are
+// read again, a few dozen of thousands.  Their elements are ranked as 64-bit
+// keys (logit, ~id), all different: ties go to the lower id, and the order of
+// the threads does not matter.  More than a buffer of them (a row of equal
+// values) are ranked by k passes instead.
 #include "kv8.cuh"
 
 #include <algorithm>
@@ -24,9 +26,10 @@ namespace {
 constexpr int kLpThreads = 256, kLpWarps = kLpThreads / 32;
 constexpr int kVecs = 4;          // 16-byte loads per thread and tile
 constexpr int kMaxTop = 64;
-constexpr int kKeep = 192;        // the candidate buffer is cut back to k above this many
-constexpr int kCap = kKeep + kMaxTop * 32;  // 64 threads at most push 32 elements each between cuts
-constexpr int kMaxMerge = 2048;   // candidates that the last CTA of a row merges
+constexpr int kGroups = 32;       // groups of a thread's tiles, at most
+constexpr int kHits = 1024;       // groups that are read again
+constexpr int kCap = 1024;        // candidates that are ranked against each other
+constexpr int kMaxMerge = kCap;   // candidates that the last CTA of a row merges
 
 typedef unsigned long long u64;
 
@@ -71,6 +74,14 @@ __device__ __forceinline__ float lp_max_nan(float a, float b)
 {
     float y;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+
+// Largest of the warp's values (NaN counts as none).
+__device__ __forceinline__ float warp_max(float x)
+{
+    float y;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
     return y;
 }
 
@@ -137,27 +148,26 @@ __device__ __forceinline__ float vec_max(const uint4& v)
 struct LpShared {
     u64 buf[kCap];
     u64 tops[kMaxTop];
-    u64 thread_max[kLpThreads];
-    u64 thr;
-    int count, last;
+    u64 best[kLpWarps];
+    float low[kLpWarps];
+    int count, hits, last;
     Sums sums[kLpWarps];
+    uint16_t hit[kHits];  // group * threads + thread
+    float group_max[1];  // [group][thread]
 };
 
-// The buffer's k best to its front, in order; its threshold.  All threads.
-__device__ __forceinline__ void cut(LpShared& z, int n, int k)
+// The k largest of the buffer's n keys to z.tops, in order (0 where there are
+// fewer).  All threads.
+__device__ __forceinline__ void rank_keys(LpShared& z, int n, int k)
 {
-    const int keep = min(n, k);
+    for (int i = threadIdx.x; i < k; i += kLpThreads)
+        if (i >= n) z.tops[i] = 0;
     for (int i = threadIdx.x; i < n; i += kLpThreads) {
         const u64 key = z.buf[i];
         int rank = 0;
-        for (int j = 0; j < n; ++j) rank += z.buf[j] > key;
-        if (rank < keep) z.tops[rank] = key;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < keep; i += kLpThreads) z.buf[i] = z.tops[i];
-    if (threadIdx.x == 0) {
-        z.count = keep;
-        if (n >= k) z.thr = z.tops[k - 1];
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) rank += z.buf[j] > key || (z.buf[j] == key && j < i);  // 0 may repeat
+        if (rank < k) z.tops[rank] = key;
     }
     __syncthreads();
 }
@@ -166,9 +176,10 @@ template <typename T>
 __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LpArgs a)
 {
     constexpr int VE = Vec<T>::n;
-    __shared__ LpShared z;
+    extern __shared__ __align__(16) uint8_t raw[];
+    LpShared& z = *reinterpret_cast<LpShared*>(raw);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    if (tid == 0) z.thr = 0, z.count = 0;
+    if (tid == 0) z.count = z.hits = 0;
     pdl_wait();
     const int row = blockIdx.x / a.split, slice = blockIdx.x % a.split;
     const T* x = static_cast<const T*>(a.x) + row * a.ldl;
@@ -184,7 +195,10 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LpArgs a)
     const uint4 none = make_uint4(ninf, ninf, ninf, ninf);
 
     Sums st{-INFINITY, 0.0f, 0.0f};
-    float thr_val = -INFINITY;
+    // Tiles of a group: as few as keep the groups within kGroups.
+    const int gt = (tiles + kGroups - 1) / kGroups;
+    float gmax = -INFINITY;
+    int left = gt, group = 0;
     uint4 nxt[kVecs];
     auto fetch = [&](int t) {
 #pragma unroll
@@ -251,51 +265,85 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LpArgs a)
         st.s += s0 + s1;
         st.e += e0 + e1;
 
-        if (a.k == 0) continue;
-        const bool hit = mt > -INFINITY && mt >= thr_val;
-        const int hits = __syncthreads_count(hit);
-        if (hits == 0) continue;
-        // Calls g with the key of each element.
-        auto each_key = [&](auto&& g) {
-            if (ragged) {
-                g(lp_key(extra, tid < head ? tid : a.V - tail + (tid - head)));
-                return;
-            }
-#pragma unroll 1
-            for (int v = 0; v < kVecs; ++v) {
-                float f[VE];
-                unpack<T>(v == 0 ? cur[0] : v == 1 ? cur[1] : v == 2 ? cur[2] : cur[3], f);
-                const int id = head + (v0 + (t * kVecs + v) * kLpThreads + tid) * VE;
-#pragma unroll
-                for (int i = 0; i < VE; ++i) g(lp_key(f[i], id + i));
-            }
-        };
-        u64 above = z.thr;
-        if (hits > kMaxTop) {
-            // The k-th best of the threads' best: a threshold for this tile.
-            u64 best = 0;
-            if (hit) each_key([&](u64 key) { best = max(best, key); });
-            z.thread_max[tid] = best;
-            __syncthreads();
-            int rank = 0;
-            for (int j = 0; j < kLpThreads; ++j) rank += z.thread_max[j] > best;
-            if (rank == a.k - 1 && best > 0) z.thr = max(above, best - 1);
-            __syncthreads();
-            above = z.thr;
+        gmax = fmaxf(gmax, mt);
+        if (--left == 0) {
+            if (a.k) z.group_max[group * kLpThreads + tid] = gmax;
+            gmax = -INFINITY, left = gt, ++group;
         }
-        if (hit)
-            each_key([&](u64 key) {
-                if (key > above) z.buf[atomicAdd(&z.count, 1)] = key;
-            });
-        __syncthreads();
-        const int n = z.count;
-        if (n > kKeep) cut(z, n, a.k);
-        const u64 thr = z.thr;
-        thr_val = thr ? lp_value(thr) : -INFINITY;
     }
     if (a.k) {
+        if (left < gt) z.group_max[group++ * kLpThreads + tid] = gmax;
+        // A threshold that at least k elements of the slice reach, if there are
+        // k above -inf at all.
+        float mine = st.m, low = -INFINITY;
+        for (int i = (a.k + kLpWarps - 1) / kLpWarps; i; --i) {
+            low = warp_max(mine);
+            const unsigned who = __ballot_sync(~0u, mine == low);
+            if (lane == __ffs(who) - 1) mine = -INFINITY;
+        }
+        if (lane == 0) z.low[warp] = low;
         __syncthreads();
-        cut(z, z.count, a.k);
+        low = z.low[0];
+        for (int w = 1; w < kLpWarps; ++w) low = fminf(low, z.low[w]);
+        // Calls g with the keys of vector i (of kVecs * gt) of a group's thread.
+        auto keys_of = [&](int q, int th, int i, auto&& g) {
+            const int t = q * gt + i / kVecs;
+            if (t == whole && ends && i % kVecs == 0) {
+                if (th >= head + tail) return;
+                const int id = th < head ? th : a.V - tail + (th - head);
+                const float y = to_f<T>(x[id]);
+                if (y >= low) g(lp_key(y, id));
+            } else if (t < whole) {
+                const int v = v0 + (t * kVecs + i % kVecs) * kLpThreads + th;
+                if (v >= v1) return;
+                float f[VE];
+                unpack<T>(xv[v], f);
+#pragma unroll
+                for (int j = 0; j < VE; ++j)
+                    if (f[j] >= low) g(lp_key(f[j], head + v * VE + j));
+            }
+        };
+        if (st.m >= low && st.m > -INFINITY)
+            for (int q = 0; q < group; ++q)
+                if (z.group_max[q * kLpThreads + tid] >= low) {
+                    const int at = atomicAdd(&z.hits, 1);
+                    if (at < kHits) z.hit[at] = (uint16_t)(q * kLpThreads + tid);
+                }
+        __syncthreads();
+        const int hits = z.hits;
+        if (hits <= kHits)
+            for (int i = tid; i < hits * kVecs * gt; i += kLpThreads) {
+                const int h = z.hit[i / (kVecs * gt)];
+                keys_of(h / kLpThreads, h % kLpThreads, i % (kVecs * gt), [&](u64 key) {
+                    if (!key) return;
+                    const int at = atomicAdd(&z.count, 1);
+                    if (at < kCap) z.buf[at] = key;
+                });
+            }
+        __syncthreads();
+        const int n = z.count;
+        if (hits <= kHits && n <= kCap) {
+            rank_keys(z, n, a.k);
+        } else {
+            u64 last = ~0ull;
+            for (int i = 0; i < a.k; ++i) {
+                u64 best = 0;
+                for (int q = 0; q < group; ++q)
+                    if (z.group_max[q * kLpThreads + tid] >= low)
+                        for (int j = 0; j < kVecs * gt; ++j)
+                            keys_of(q, tid, j, [&](u64 key) {
+                                if (key < last && key > best) best = key;
+                            });
+                for (int d = 16; d; d >>= 1) best = max(best, __shfl_xor_sync(~0u, best, d));
+                if (lane == 0) z.best[warp] = best;
+                __syncthreads();
+                for (int w = 0; w < kLpWarps; ++w) best = max(best, z.best[w]);
+                __syncthreads();
+                if (tid == 0) z.tops[i] = best;
+                last = best;
+            }
+            __syncthreads();
+        }
     }
     // The row's sums: over the warp, the CTA, the slices.
     for (int d = 16; d; d >>= 1) {
@@ -313,7 +361,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LpArgs a)
     if (a.split > 1) {
         const size_t at = (size_t)row * a.split;
         if (tid == 0) a.part[at + slice] = make_float4(st.m, st.s, st.e, 0.0f);
-        for (int i = tid; i < a.k; i += kLpThreads) a.keys[(at + slice) * a.k + i] = i < z.count ? z.buf[i] : 0;
+        for (int i = tid; i < a.k; i += kLpThreads) a.keys[(at + slice) * a.k + i] = z.tops[i];
         __threadfence();
         __syncthreads();
         if (tid == 0) {
@@ -331,7 +379,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LpArgs a)
         if (a.k) {
             for (int i = tid; i < a.split * a.k; i += kLpThreads) z.buf[i] = __ldcg(a.keys + at * a.k + i);
             __syncthreads();
-            cut(z, a.split * a.k, a.k);
+            rank_keys(z, a.split * a.k, a.k);
         }
     }
     constexpr float ln2 = 0.693147180559945f;
@@ -352,7 +400,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LpArgs a)
         }
     }
     for (int i = tid; i < a.k; i += kLpThreads) {
-        const u64 key = i < z.count ? z.buf[i] : 0;
+        const u64 key = z.tops[i];
         if (a.top_id) a.top_id[(size_t)row * a.k + i] = key ? (int)~(uint32_t)key : -1;
         if (a.top_lp) a.top_lp[(size_t)row * a.k + i] = bad ? NAN : key ? lp_value(key) * a.inv_t - lse : -INFINITY;
     }
@@ -431,7 +479,11 @@ int quantr_logprobs_dev(const void* x, long long ldl, uint32_t type, int rows, i
     c.stream = (cudaStream_t)stream;
     return kv8_done(with_type(type, [&](auto* t) {
         using T = std::remove_const_t<std::remove_pointer_t<decltype(t)>>;
-        return launch_ex(k_logprobs<T>, dim3((unsigned)(rows * a.split)), kLpThreads, 0, c, a);
+        // Tiles of the longest slice, with one for the ragged ends.
+        const int vecs = vocab / Vec<T>::n, per = (vecs + a.split - 1) / a.split;
+        const int tiles = (per + kVecs * kLpThreads - 1) / (kVecs * kLpThreads) + 1;
+        const size_t smem = sizeof(LpShared) + (k ? std::min(tiles, kGroups) * kLpThreads * sizeof(float) : 0);
+        return launch_ex(k_logprobs<T>, dim3((unsigned)(rows * a.split)), kLpThreads, smem, c, a);
     }));
 }
 
