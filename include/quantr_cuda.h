@@ -553,7 +553,9 @@ int quantr_kv8_read_dev(void* k, long long ldk, void* v, long long ldv, uint32_t
  * missing counts as masked.  A query or a scale that is not finite gives NaN.
  * max_len is the longest sequence expected: it sizes the split of long
  * sequences over the GPU and the workspace; longer ones are right, only
- * slower.  The workspace must be 256-byte aligned. */
+ * slower.  The workspace must be 256-byte aligned and its first 4096 bytes zero
+ * before its first use; every call leaves them zero, so it is zeroed once.
+ * Calls that may overlap need a workspace each. */
 size_t quantr_kv8_attend_workspace_bytes(const quantr_kv8_pool* pool, const quantr_kv8_batch* batch, int n_heads,
                                          int max_len);
 int quantr_kv8_attend_dev(void* out, long long ldo, const void* q, long long ldq, uint32_t type, int n_heads,
@@ -604,8 +606,9 @@ int quantr_kv8_copy_pages_dev(const quantr_kv8_pool* pool, const int* dst, const
  * Each output may be NULL (token too, with logprob).  Logits of -inf have
  * probability 0.  A row of nothing else gives lse = -inf, logprob = -inf,
  * entropy = 0; one with a NaN or +inf gives NaN in all three and in
- * top_logprob (its top_id are the k largest that are not NaN).  The workspace
- * must be 256-byte aligned. */
+ * top_logprob (its top_id are the k largest that are not NaN).  No workspace is
+ * needed today (quantr_logprobs_workspace_bytes is 0: pass any pointer or
+ * NULL). */
 size_t quantr_logprobs_workspace_bytes(int rows, int vocab, int k);
 int quantr_logprobs_dev(const void* x, long long ldl, uint32_t type, int rows, int vocab, float temperature,
                         const int* token, float* logprob, float* entropy, float* lse, int k, int* top_id,

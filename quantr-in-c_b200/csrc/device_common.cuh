@@ -208,6 +208,31 @@ __device__ __forceinline__ void cp_wait()
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+// Cluster barrier halves, and the shared-window address of `p` in the cluster's
+// CTA `rank` (for the remote accesses below).
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t remote_of(const void* p, uint32_t rank)
+{
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(sptr(p)), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ void st_remote(uint32_t a, float v)
+{
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory");
+}
+__device__ __forceinline__ void st_remote(uint32_t a, unsigned long long v)
+{
+    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(v) : "memory");
+}
+__device__ __forceinline__ int add_remote(uint32_t a, int v)
+{
+    int r;
+    asm volatile("atom.shared::cluster.add.s32 %0, [%1], %2;" : "=r"(r) : "r"(a), "r"(v) : "memory");
+    return r;
+}
+
 // dp4a with unsigned bytes in `a` and signed bytes in `b`.
 __device__ __forceinline__ int dp4a_us(uint32_t a, int b, int c)
 {

@@ -9,12 +9,13 @@
 //
 // Alternatives cost the pass nothing but a store: a thread keeps the maximum of
 // each group of its elements, which the softmax needs anyway.  Then a threshold
-// that k elements reach at least (each warp's ceil(k/8)-th largest thread
-// maximum, the least of the 8 warps), and only the groups that reach it are
-// read again, a few dozen of thousands.  Their elements are ranked as 64-bit
-// keys (logit, ~id), all different: ties go to the lower id, and the order of
-// the threads does not matter.  More than a buffer of them (a row of equal
-// values) are ranked by k passes instead.
+// that k elements of the row reach at least (the k-th largest of every warp's
+// few largest thread maxima), and only the groups that reach it are read again,
+// about k of thousands.  Their elements are ranked as 64-bit keys (logit, ~id), all different: ties go to
+// the lower id, and the order of the threads does not matter.
+//
+// A row is one CTA, or a cluster of up to 8 where there are few rows, joined
+// through distributed shared memory.
 #include "kv8.cuh"
 
 #include <algorithm>
@@ -27,9 +28,10 @@ constexpr int kLpThreads = 256, kLpWarps = kLpThreads / 32;
 constexpr int kVecs = 4;          // 16-byte loads per thread and tile
 constexpr int kMaxTop = 64;
 constexpr int kGroups = 32;       // groups of a thread's tiles, at most
+constexpr int kMaxHeads = 128;    // values that the threshold is chosen from
 constexpr int kHits = 1024;       // groups that are read again
 constexpr int kCap = 1024;        // candidates that are ranked against each other
-constexpr int kMaxMerge = kCap;   // candidates that the last CTA of a row merges
+constexpr int kMaxSplit = 8;      // CTAs of a row: one cluster
 
 typedef unsigned long long u64;
 
@@ -44,9 +46,6 @@ struct LpArgs {
     float* lse;
     int* top_id;
     float* top_lp;
-    int* counters;  // one per row, zero between calls
-    float4* part;   // (m, s, e) of every (row, slice)
-    u64* keys;      // k of every (row, slice)
 };
 
 // Order of alternatives: larger logits first, then lower ids.  0 is below all
@@ -107,6 +106,33 @@ struct Vec {
     static constexpr int n = 16 / sizeof(T);
 };
 
+// Two floats that one instruction works on (fma/add.rn.f32x2).
+struct F2 {
+    u64 v;
+};
+__device__ __forceinline__ F2 f2(float a, float b)
+{
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void f2_get(F2 x, float& a, float& b)
+{
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v));
+}
+__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c)
+{
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+__device__ __forceinline__ F2 f2_add(F2 a, F2 b)
+{
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+
 // Elements of one 16-byte load.
 template <typename T>
 __device__ __forceinline__ void unpack(const uint4& v, float* x)
@@ -124,6 +150,45 @@ __device__ __forceinline__ void unpack(const uint4& v, float* x)
             x[2 * i] = f.x;
             x[2 * i + 1] = f.y;
         }
+    }
+}
+
+// The bound below which the fast path takes logits as one: 2^-200 of the
+// maximum or less, so that their weight is 0 either way, and -inf makes no
+// 0 * -inf.
+template <typename T>
+struct Low {
+    static constexpr float bound = -1e30f;
+};
+template <>
+struct Low<__half> {
+    static constexpr float bound = -65504.0f;
+};
+
+// The same elements, not below the bound; NaN stays NaN.
+template <typename T>
+__device__ __forceinline__ void unpack_bounded(const uint4& v, float* x)
+{
+    if constexpr (sizeof(T) == 4) {
+        unpack<T>(v, x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = lp_max_nan(x[i], Low<T>::bound);
+    } else {
+        uint4 u = v;
+        uint32_t* w = &u.x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (std::is_same_v<T, __half>) {
+                const __half2 b = __float2half2_rn(Low<T>::bound);
+                const __half2 h = __hmax2_nan(*reinterpret_cast<const __half2*>(&w[i]), b);
+                w[i] = *reinterpret_cast<const uint32_t*>(&h);
+            } else {
+                const __nv_bfloat162 b = __float2bfloat162_rn(Low<T>::bound);
+                const __nv_bfloat162 h = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&w[i]), b);
+                w[i] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+        }
+        unpack<T>(u, x);
     }
 }
 
@@ -146,14 +211,15 @@ __device__ __forceinline__ float vec_max(const uint4& v)
 }
 
 struct LpShared {
-    u64 buf[kCap];
+    u64 buf[kCap];  // of the row's first CTA, as are count and part
     u64 tops[kMaxTop];
     u64 best[kLpWarps];
-    float low[kLpWarps];
-    int count, hits, last;
-    Sums sums[kLpWarps];
+    float heads[kMaxHeads];  // every warp's largest thread maxima, of the whole row
+    float low;
+    Sums part[kMaxSplit], sums[kLpWarps];
+    int count, hits;
     uint16_t hit[kHits];  // group * threads + thread
-    float group_max[1];  // [group][thread]
+    float group_max[1];   // [group][thread]
 };
 
 // The k largest of the buffer's n keys to z.tops, in order (0 where there are
@@ -166,8 +232,55 @@ __device__ __forceinline__ void rank_keys(LpShared& z, int n, int k)
         const u64 key = z.buf[i];
         int rank = 0;
 #pragma unroll 8
-        for (int j = 0; j < n; ++j) rank += z.buf[j] > key || (z.buf[j] == key && j < i);  // 0 may repeat
+        for (int j = 0; j < n; ++j) rank += z.buf[j] > key;
         if (rank < k) z.tops[rank] = key;
+    }
+    __syncthreads();
+}
+
+// More candidates than the buffer holds: the k best of the row with those above
+// `low`, then of those equal to it the first ones; k passes where even the
+// former are too many.  By the row's first CTA.
+template <typename T>
+__device__ __noinline__ void crowded(const LpArgs& a, LpShared& z, const T* x, float low)
+{
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    __syncthreads();
+    if (tid == 0) z.count = 0;
+    __syncthreads();
+    for (int v = tid; v < a.V; v += kLpThreads) {
+        const float y = to_f<T>(x[v]);
+        if (!(y > low)) continue;
+        const int i = atomicAdd(&z.count, 1);
+        if (i < kCap) z.buf[i] = lp_key(y, v);
+    }
+    __syncthreads();
+    int n = z.count;
+    if (n <= kCap - kLpThreads) {
+        for (int v0 = 0; v0 < a.V && n < a.k && low > -INFINITY; v0 += kLpThreads) {
+            const int v = v0 + tid;
+            __syncthreads();
+            if (v < a.V && to_f<T>(x[v]) == low) z.buf[atomicAdd(&z.count, 1)] = lp_key(low, v);
+            __syncthreads();
+            n = z.count;
+        }
+        rank_keys(z, n, a.k);
+        return;
+    }
+    u64 last = ~0ull;
+    for (int i = 0; i < a.k; ++i) {
+        u64 best = 0;
+        for (int v = tid; v < a.V; v += kLpThreads) {
+            const u64 key = lp_key(to_f<T>(x[v]), v);
+            if (key < last && key > best) best = key;
+        }
+        for (int d = 16; d; d >>= 1) best = max(best, __shfl_xor_sync(~0u, best, d));
+        if (lane == 0) z.best[warp] = best;
+        __syncthreads();
+        for (int w = 0; w < kLpWarps; ++w) best = max(best, z.best[w]);
+        __syncthreads();
+        if (tid == 0) z.tops[i] = best;
+        last = best;
     }
     __syncthreads();
 }
@@ -179,7 +292,8 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LpArgs a)
     extern __shared__ __align__(16) uint8_t raw[];
     LpShared& z = *reinterpret_cast<LpShared*>(raw);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    if (tid == 0) z.count = z.hits = 0;
+    if (tid == 0) z.count = z.hits = 0, z.low = -INFINITY;
+    cluster_arrive();  // every CTA of the cluster has begun, and zeroed its counts: waited for before the first remote access
     pdl_wait();
     const int row = blockIdx.x / a.split, slice = blockIdx.x % a.split;
     const T* x = static_cast<const T*>(a.x) + row * a.ldl;
@@ -189,8 +303,8 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LpArgs a)
     const int per = (nvec + a.split - 1) / a.split, v0 = min(nvec, slice * per), v1 = min(nvec, v0 + per);
     const uint4* xv = reinterpret_cast<const uint4*>(x + head);
     const bool ends = (head | tail) && slice == a.split - 1;  // the last slice takes the ragged ends too
-    const int tiles = (v1 - v0 + kVecs * kLpThreads - 1) / (kVecs * kLpThreads) + (ends ? 1 : 0);
-    const int whole = tiles - (ends ? 1 : 0);
+    const int full = (v1 - v0) / (kVecs * kLpThreads);        // tiles without a bound to look at
+    const int whole = (v1 - v0 + kVecs * kLpThreads - 1) / (kVecs * kLpThreads), tiles = whole + (ends ? 1 : 0);
     const uint32_t ninf = sizeof(T) == 4 ? 0xff800000u : std::is_same_v<T, __half> ? 0xfc00fc00u : 0xff80ff80u;
     const uint4 none = make_uint4(ninf, ninf, ninf, ninf);
 
@@ -199,26 +313,9 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LpArgs a)
     const int gt = (tiles + kGroups - 1) / kGroups;
     float gmax = -INFINITY;
     int left = gt, group = 0;
-    uint4 nxt[kVecs];
-    auto fetch = [&](int t) {
-#pragma unroll
-        for (int i = 0; i < kVecs; ++i) {
-            const int v = v0 + (t * kVecs + i) * kLpThreads + tid;
-            nxt[i] = t < whole && v < v1 ? __ldcs(xv + v) : none;
-        }
-    };
-    fetch(0);
-    for (int t = 0; t < tiles; ++t) {
-        uint4 cur[kVecs];
-#pragma unroll
-        for (int i = 0; i < kVecs; ++i) cur[i] = nxt[i];
-        fetch(t + 1);
-        const bool ragged = t == whole;  // one element per thread: head, then tail
-        float extra = -INFINITY;
-        if (ragged && tid < head + tail) extra = to_f<T>(x[tid < head ? tid : a.V - tail + (tid - head)]);
-        float mt = extra;
-#pragma unroll
-        for (int i = 0; i < kVecs; ++i) mt = fmaxf(mt, vec_max<T>(cur[i]));
+    const F2 c2 = f2(a.c, a.c);
+    // The running maximum takes `mt` in; the group's, too.
+    auto raise = [&](float mt) {
         if (mt > st.m) {
             if (st.m > -INFINITY) {
                 const float d = (st.m - mt) * a.c, r = lp_ex2(d);
@@ -227,33 +324,50 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LpArgs a)
             }
             st.m = mt;
         }
-        const float ref = st.m == -INFINITY ? 0.0f : st.m * a.c;
-        float s0 = 0.0f, s1 = 0.0f, e0 = 0.0f, e1 = 0.0f;
-        if (fabsf(ref) <= 3.402823466e38f && !ragged) {
+        gmax = fmaxf(gmax, mt);
+        if (--left == 0) {
+            if (a.k) z.group_max[group * kLpThreads + tid] = gmax;
+            gmax = -INFINITY, left = gt, ++group;
+        }
+    };
+    auto one = [&](float y) {
+        const float base = st.m == -INFINITY ? 0.0f : st.m;
+        // 2^-200 is 0; the bound keeps -inf out of 0 * -inf and NaN in.
+        const float d = lp_max_nan((y - base) * a.c, -200.0f), p = lp_ex2(d);
+        st.s += p;
+        st.e = fmaf(p, d, st.e);
+    };
+    auto take = [&](const uint4 (&cur)[kVecs]) {
+        float mt = vec_max<T>(cur[0]);
+#pragma unroll
+        for (int i = 1; i < kVecs; ++i) mt = fmaxf(mt, vec_max<T>(cur[i]));
+        raise(mt);
+        if (fabsf(st.m * a.c) <= 3.402823466e38f && (st.m - Low<T>::bound) * a.c > 200.0f) {
+            const float ref = -st.m * a.c;
+            const F2 r2 = f2(ref, ref);
+            F2 s2 = f2(0.0f, 0.0f), e2 = s2;
 #pragma unroll
             for (int v = 0; v < kVecs; ++v) {
                 float f[VE];
-                unpack<T>(cur[v], f);
+                unpack_bounded<T>(cur[v], f);
 #pragma unroll
                 for (int i = 0; i < VE; i += 2) {
-                    // 2^-200 is 0; the bound keeps -inf out of 0 * -inf and NaN in.
-                    const float d0 = lp_max_nan(fmaf(f[i], a.c, -ref), -200.0f);
-                    const float d1 = lp_max_nan(fmaf(f[i + 1], a.c, -ref), -200.0f);
-                    const float p0 = lp_ex2(d0), p1 = lp_ex2(d1);
-                    s0 += p0, s1 += p1;
-                    e0 = fmaf(p0, d0, e0), e1 = fmaf(p1, d1, e1);
+                    const F2 d = f2_fma(f2(f[i], f[i + 1]), c2, r2);
+                    float d0, d1;
+                    f2_get(d, d0, d1);
+                    const F2 p = f2(lp_ex2(d0), lp_ex2(d1));
+                    s2 = f2_add(s2, p);
+                    e2 = f2_fma(p, d, e2);
                 }
             }
+            float x0, x1;
+            f2_get(s2, x0, x1);
+            st.s += x0 + x1;
+            f2_get(e2, x0, x1);
+            st.e += x0 + x1;
         } else {
-            // The ragged ends, and maxima so large that c times them has no
-            // float (a row of nothing but the type's lowest value, say).
-            const float base = st.m == -INFINITY ? 0.0f : st.m;
-            auto one = [&](float y) {
-                const float d = lp_max_nan((y - base) * a.c, -200.0f), p = lp_ex2(d);
-                s0 += p;
-                e0 = fmaf(p, d, e0);
-            };
-            one(extra);
+            // Nothing above the bound yet, or a maximum that c times has no
+            // float: a row of nothing but the type's lowest value, say.
 #pragma unroll 1
             for (int v = 0; v < kVecs; ++v) {
                 float f[VE];
@@ -262,126 +376,143 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LpArgs a)
                 for (int i = 0; i < VE; ++i) one(f[i]);
             }
         }
-        st.s += s0 + s1;
-        st.e += e0 + e1;
-
-        gmax = fmaxf(gmax, mt);
-        if (--left == 0) {
-            if (a.k) z.group_max[group * kLpThreads + tid] = gmax;
-            gmax = -INFINITY, left = gt, ++group;
+    };
+    // Two tiles in flight.
+    const uint4* at = xv + v0 + tid;
+    auto fetch = [&](uint4 (&buf)[kVecs], int t) {
+        if (t < full) {
+            const uint4* p = at + (size_t)t * (kVecs * kLpThreads);
+#pragma unroll
+            for (int i = 0; i < kVecs; ++i) buf[i] = __ldcs(p + i * kLpThreads);
+        }
+    };
+    {
+        uint4 b0[kVecs], b1[kVecs];
+        fetch(b0, 0);
+        fetch(b1, 1);
+        for (int t = 0; t < full; t += 2) {
+            take(b0);
+            fetch(b0, t + 2);
+            if (t + 1 < full) {
+                take(b1);
+                fetch(b1, t + 3);
+            }
+        }
+        if (whole > full) {
+#pragma unroll
+            for (int i = 0; i < kVecs; ++i) {
+                const int v = v0 + (full * kVecs + i) * kLpThreads + tid;
+                b0[i] = v < v1 ? __ldcs(xv + v) : none;
+            }
+            take(b0);
         }
     }
+    if (ends) {  // one element per thread: head, then tail
+        const float y = tid < head + tail ? to_f<T>(x[tid < head ? tid : a.V - tail + (tid - head)]) : -INFINITY;
+        raise(y);
+        if (tid < head + tail) one(y);
+    }
+    // Warps that the threshold looks at: all of them, or those that a short row
+    // fills (a split row's slices are long).
+    const int nw = a.split > 1 ? kLpWarps : max(1, min(kLpWarps, nvec / 32));
+    // The row's sums: over the warp, the CTA, the cluster.
+    Sums mine = st;
+    for (int d = 16; d; d >>= 1) {
+        Sums o;
+        o.m = __shfl_xor_sync(~0u, mine.m, d);
+        o.s = __shfl_xor_sync(~0u, mine.s, d);
+        o.e = __shfl_xor_sync(~0u, mine.e, d);
+        mine = lane & d ? join(o, mine, a.c) : join(mine, o, a.c);  // the same operands in the same order on both lanes
+    }
+    if (lane == 0) z.sums[warp] = mine;
+    // Each warp's `per_warp` largest thread maxima, told to every CTA of the row.
+    const int heads = nw * a.split, per_warp = a.k ? min((a.k + heads - 1) / heads + 1, min(32, kMaxHeads / heads)) : 0;
+    float y = st.m, head_val = -INFINITY;
+    if (a.k && left < gt) z.group_max[group++ * kLpThreads + tid] = gmax;
+    for (int i = 0; i < per_warp && warp < nw; ++i) {
+        const float top = warp_max(y);
+        const unsigned who = __ballot_sync(~0u, y == top);
+        if (lane == __ffs(who) - 1) y = -INFINITY;
+        if (lane == i) head_val = top;
+    }
+    __syncthreads();
+    cluster_wait();
+    if (warp < nw && lane < per_warp)
+        for (int r = 0; r < a.split; ++r)
+            st_remote(remote_of(&z.heads[(slice * nw + warp) * per_warp + lane], r), head_val);
+    if (tid == 0) {
+        Sums t = z.sums[0];
+        for (int w = 1; w < kLpWarps; ++w) t = join(t, z.sums[w], a.c);
+        st_remote(remote_of(&z.part[slice].m, 0), t.m);
+        st_remote(remote_of(&z.part[slice].s, 0), t.s);
+        st_remote(remote_of(&z.part[slice].e, 0), t.e);
+    }
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
     if (a.k) {
-        if (left < gt) z.group_max[group++ * kLpThreads + tid] = gmax;
-        // A threshold that at least k elements of the slice reach, if there are
-        // k above -inf at all.
-        float mine = st.m, low = -INFINITY;
-        for (int i = (a.k + kLpWarps - 1) / kLpWarps; i; --i) {
-            low = warp_max(mine);
-            const unsigned who = __ballot_sync(~0u, mine == low);
-            if (lane == __ffs(who) - 1) mine = -INFINITY;
+        // The k-th largest of them, which k of the row's elements reach; none
+        // where a short row has fewer.
+        const int n = heads * per_warp;
+        if (tid < n) {
+            const float v = z.heads[tid];
+            int rank = 0;
+#pragma unroll 8
+            for (int i = 0; i < n; ++i) rank += z.heads[i] > v || (z.heads[i] == v && i < tid);
+            if (rank == a.k - 1) z.low = v;
         }
-        if (lane == 0) z.low[warp] = low;
         __syncthreads();
-        low = z.low[0];
-        for (int w = 1; w < kLpWarps; ++w) low = fminf(low, z.low[w]);
-        // Calls g with the keys of vector i (of kVecs * gt) of a group's thread.
-        auto keys_of = [&](int q, int th, int i, auto&& g) {
-            const int t = q * gt + i / kVecs;
-            if (t == whole && ends && i % kVecs == 0) {
-                if (th >= head + tail) return;
-                const int id = th < head ? th : a.V - tail + (th - head);
-                const float y = to_f<T>(x[id]);
-                if (y >= low) g(lp_key(y, id));
-            } else if (t < whole) {
-                const int v = v0 + (t * kVecs + i % kVecs) * kLpThreads + th;
-                if (v >= v1) return;
-                float f[VE];
-                unpack<T>(xv[v], f);
-#pragma unroll
-                for (int j = 0; j < VE; ++j)
-                    if (f[j] >= low) g(lp_key(f[j], head + v * VE + j));
+        const float low = z.low;
+        const uint32_t count = remote_of(&z.count, 0), buf = remote_of(z.buf, 0);
+        auto push = [&](float y, int id) {
+            if (!(y >= low && y > -INFINITY)) return;
+            if (a.split == 1) {
+                const int i = atomicAdd(&z.count, 1);
+                if (i < kCap) z.buf[i] = lp_key(y, id);
+            } else {
+                const int i = add_remote(count, 1);
+                if (i < kCap) st_remote(buf + 8 * i, lp_key(y, id));
             }
         };
         if (st.m >= low && st.m > -INFINITY)
             for (int q = 0; q < group; ++q)
                 if (z.group_max[q * kLpThreads + tid] >= low) {
-                    const int at = atomicAdd(&z.hits, 1);
-                    if (at < kHits) z.hit[at] = (uint16_t)(q * kLpThreads + tid);
+                    const int i = atomicAdd(&z.hits, 1);
+                    if (i < kHits) z.hit[i] = (uint16_t)(q * kLpThreads + tid);
                 }
         __syncthreads();
-        const int hits = z.hits;
-        if (hits <= kHits)
-            for (int i = tid; i < hits * kVecs * gt; i += kLpThreads) {
-                const int h = z.hit[i / (kVecs * gt)];
-                keys_of(h / kLpThreads, h % kLpThreads, i % (kVecs * gt), [&](u64 key) {
-                    if (!key) return;
-                    const int at = atomicAdd(&z.count, 1);
-                    if (at < kCap) z.buf[at] = key;
-                });
+        const int hits = min(z.hits, kHits);
+        if (z.hits > kHits && tid == 0) add_remote(count, kCap + 1);
+        for (int i = tid; i < hits * kVecs * gt; i += kLpThreads) {
+            // Vector i % (kVecs * gt) of the group.
+            const int h = z.hit[i / (kVecs * gt)], j = i % (kVecs * gt), th = h % kLpThreads;
+            const int t = h / kLpThreads * gt + j / kVecs;
+            if (t < whole) {
+                const int v = v0 + (t * kVecs + j % kVecs) * kLpThreads + th;
+                if (v >= v1) continue;
+                float f[VE];
+                unpack<T>(xv[v], f);
+#pragma unroll
+                for (int e = 0; e < VE; ++e) push(f[e], head + v * VE + e);
+            } else if (t < tiles && j % kVecs == 0 && th < head + tail) {
+                const int id = th < head ? th : a.V - tail + (th - head);
+                push(to_f<T>(x[id]), id);
             }
-        __syncthreads();
-        const int n = z.count;
-        if (hits <= kHits && n <= kCap) {
-            rank_keys(z, n, a.k);
+        }
+        __syncwarp();
+        cluster_arrive();
+        if (slice) return;  // nobody reads this CTA's shared memory any more
+        cluster_wait();
+        if (z.count <= kCap) {
+            rank_keys(z, z.count, a.k);
         } else {
-            u64 last = ~0ull;
-            for (int i = 0; i < a.k; ++i) {
-                u64 best = 0;
-                for (int q = 0; q < group; ++q)
-                    if (z.group_max[q * kLpThreads + tid] >= low)
-                        for (int j = 0; j < kVecs * gt; ++j)
-                            keys_of(q, tid, j, [&](u64 key) {
-                                if (key < last && key > best) best = key;
-                            });
-                for (int d = 16; d; d >>= 1) best = max(best, __shfl_xor_sync(~0u, best, d));
-                if (lane == 0) z.best[warp] = best;
-                __syncthreads();
-                for (int w = 0; w < kLpWarps; ++w) best = max(best, z.best[w]);
-                __syncthreads();
-                if (tid == 0) z.tops[i] = best;
-                last = best;
-            }
-            __syncthreads();
+            crowded<T>(a, z, x, low);
         }
+    } else if (slice) {
+        return;
     }
-    // The row's sums: over the warp, the CTA, the slices.
-    for (int d = 16; d; d >>= 1) {
-        Sums o;
-        o.m = __shfl_xor_sync(~0u, st.m, d);
-        o.s = __shfl_xor_sync(~0u, st.s, d);
-        o.e = __shfl_xor_sync(~0u, st.e, d);
-        st = lane & d ? join(o, st, a.c) : join(st, o, a.c);  // the same operands in the same order on both lanes
-    }
-    if (lane == 0) z.sums[warp] = st;
-    __syncthreads();
-    st = z.sums[0];
-    for (int w = 1; w < kLpWarps; ++w) st = join(st, z.sums[w], a.c);
-
-    if (a.split > 1) {
-        const size_t at = (size_t)row * a.split;
-        if (tid == 0) a.part[at + slice] = make_float4(st.m, st.s, st.e, 0.0f);
-        for (int i = tid; i < a.k; i += kLpThreads) a.keys[(at + slice) * a.k + i] = z.tops[i];
-        __threadfence();
-        __syncthreads();
-        if (tid == 0) {
-            z.last = atomicAdd(a.counters + row, 1) == a.split - 1;
-            if (z.last) a.counters[row] = 0;
-            __threadfence();
-        }
-        __syncthreads();
-        if (!z.last) return;
-        st = {-INFINITY, 0.0f, 0.0f};
-        for (int i = 0; i < a.split; ++i) {
-            const float4 q = __ldcg(a.part + at + i);
-            st = join(st, Sums{q.x, q.y, q.z}, a.c);
-        }
-        if (a.k) {
-            for (int i = tid; i < a.split * a.k; i += kLpThreads) z.buf[i] = __ldcg(a.keys + at * a.k + i);
-            __syncthreads();
-            rank_keys(z, a.split * a.k, a.k);
-        }
-    }
+    st = z.part[0];
+    for (int i = 1; i < a.split; ++i) st = join(st, z.part[i], a.c);
     constexpr float ln2 = 0.693147180559945f;
     const float l2 = log2f(st.s);
     const bool bad = st.s != st.s || st.m == INFINITY;
@@ -406,35 +537,12 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LpArgs a)
     }
 }
 
-// Slices per row.  One CTA streams about 9 KB per microsecond and SM while 4 of
-// them share an SM; a slice is at least two tiles.
-int lp_split(int rows, int vocab, int k)
+// CTAs per row: a row has a fixed cost (launch, threshold, ranking), so a row
+// is split only while there are fewer CTAs than two per SM.
+int lp_split(int rows, int vocab)
 {
-    const long long slots = 4ll * device_sm_count();
-    const int most = std::max(1, std::min((vocab + 8191) / 8192, k ? kMaxMerge / k : 1024));
-    if ((long long)rows * most <= slots) return most;
-    if (rows < slots) return std::max(1, (int)(slots / rows));
-    // Several waves: the split whose last wave is fullest.
-    int best = 1;
-    double fill = 0.0;
-    for (int s = 1; s <= std::min(most, 8); ++s) {
-        const long long n = (long long)rows * s, waves = (n + slots - 1) / slots;
-        const double f = (double)n / (waves * slots) - 0.01 * s;
-        if (f > fill) fill = f, best = s;
-    }
-    return best;
-}
-
-struct LpWs {
-    size_t part, keys, total;
-};
-LpWs lp_ws(int rows, int split, int k)
-{
-    LpWs w;
-    w.part = ((size_t)rows * 4 + 255) & ~size_t(255);
-    w.keys = w.part + (size_t)rows * split * sizeof(float4);
-    w.total = w.keys + (size_t)rows * split * k * sizeof(u64);
-    return w;
+    const int most = std::min(kMaxSplit, std::max(1, (vocab + 4095) / 4096));
+    return std::min(most, (2 * device_sm_count() + rows - 1) / rows);
 }
 
 } // namespace
@@ -446,8 +554,8 @@ using namespace qr;
 
 size_t quantr_logprobs_workspace_bytes(int rows, int vocab, int k)
 {
-    if (rows <= 0 || vocab <= 0 || k < 0 || k > kMaxTop) return 256;
-    return std::max<size_t>(256, lp_ws(rows, lp_split(rows, vocab, k), k).total);
+    (void)rows, (void)vocab, (void)k;
+    return 0;
 }
 
 int quantr_logprobs_dev(const void* x, long long ldl, uint32_t type, int rows, int vocab, float temperature,
@@ -461,20 +569,13 @@ int quantr_logprobs_dev(const void* x, long long ldl, uint32_t type, int rows, i
     if (k > kMaxTop) return QUANTR_ERR_TOO_LARGE;
     if (rows == 0) return QUANTR_OK;
     if (!x || (uintptr_t)x % (type == QUANTR_TYPE_F32 ? 4 : 2) || (logprob && !token)) return QUANTR_ERR_BAD_ARG;
-    if (!workspace || ((uintptr_t)workspace & 255) ||
-        workspace_bytes < quantr_logprobs_workspace_bytes(rows, vocab, k))
-        return QUANTR_ERR_WORKSPACE;
+    (void)workspace, (void)workspace_bytes;
     LpArgs a{};
-    a.x = x, a.ldl = ldl, a.rows = rows, a.V = vocab, a.k = k, a.split = lp_split(rows, vocab, k);
+    a.x = x, a.ldl = ldl, a.rows = rows, a.V = vocab, a.k = k, a.split = lp_split(rows, vocab);
     if ((long long)rows * a.split > 0x7fffffffll) return QUANTR_ERR_TOO_LARGE;
     a.inv_t = (float)(1.0 / (double)temperature);
     a.c = (float)(1.4426950408889634 / (double)temperature);
     a.token = token, a.logprob = logprob, a.entropy = entropy, a.lse = lse, a.top_id = top_id, a.top_lp = top_logprob;
-    const LpWs w = lp_ws(rows, a.split, k);
-    uint8_t* base = static_cast<uint8_t*>(workspace);
-    a.counters = reinterpret_cast<int*>(base);
-    a.part = reinterpret_cast<float4*>(base + w.part);
-    a.keys = reinterpret_cast<u64*>(base + w.keys);
     LaunchCfg c;
     c.stream = (cudaStream_t)stream;
     return kv8_done(with_type(type, [&](auto* t) {
@@ -483,7 +584,7 @@ int quantr_logprobs_dev(const void* x, long long ldl, uint32_t type, int rows, i
         const int vecs = vocab / Vec<T>::n, per = (vecs + a.split - 1) / a.split;
         const int tiles = (per + kVecs * kLpThreads - 1) / (kVecs * kLpThreads) + 1;
         const size_t smem = sizeof(LpShared) + (k ? std::min(tiles, kGroups) * kLpThreads * sizeof(float) : 0);
-        return launch_ex(k_logprobs<T>, dim3((unsigned)(rows * a.split)), kLpThreads, smem, c, a);
+        return launch_cluster(k_logprobs<T>, dim3((unsigned)(rows * a.split)), kLpThreads, smem, a.split, c, a);
     }));
 }
 
