@@ -41,8 +41,11 @@ namespace {
 
 constexpr int kThreads = 320;
 constexpr int kTile = 128;     // tokens per tile
-constexpr int kMeta = 16;      // ring of per-tile page scales
+constexpr int kMeta = 16;      // rings of the segments, and of the tiles' page scales
 constexpr int kMaxStages = 6;
+constexpr int kChunk = 32;     // parts of a row tile joined at once
+constexpr int kGroup = 16;     // more of them than kChunk are joined in groups first
+constexpr int kMaxCtas = 512;
 
 struct AttendParams {
     CUtensorMap kmap, vmap;
@@ -53,9 +56,11 @@ struct AttendParams {
     long long ldq, ldo;
     uint32_t type;
     int H, G, window;
+    unsigned inv_g;  // ceil(2^32 / G): f / G = umulhi(f, inv_g) for f * G < 2^32 (G = 1 apart)
     float scale2;  // scale * log2(e)
+    int vec;       // query rows allow aligned loads of four
     int stages, nS, nO, tmem_cols, min_share;
-    int* counters;  // one per CTA, zero between calls
+    int* counters;  // [2][kMaxCtas] by a row tile's (a group's) first CTA, zero between calls
     float* part;    // 2 per CTA: o [RT][128], m [RT], l [RT]
 };
 
@@ -149,99 +154,107 @@ __device__ __forceinline__ float max_nan(float a, float b)
 
 // ---------------------------------------------------------------- the walk --
 
-// The segments (runs of tiles of one row tile) of this CTA's share, walked by
-// every warp for itself; all values are uniform over the warp.
-struct Walk {
-    long long pos, end, share;  // flat tiles
-    long long first;            // flat index of sequence b's first tile
-    int b, nrt, nt, tlo;        // row tiles, token tiles, first token tile of the sequence
-    long long cnt;
-    Kv8Seq s;
-    // current segment
-    int h, rt, t0, t1;
-    long long item0;  // flat index of the row tile's first tile
+// One segment: a run of 128-token tiles of one row tile.  c0, c1: the first and
+// last CTA that have a part of the row tile.
+struct Seg {
+    int h, rt, row0, n, len;  // KV head, row tile; the sequence's first row, rows, length
+    int t0, t1, c0, c1;       // t1 = t0: no more segments
 };
 
+// The copying warp walks this CTA's share; all values are uniform over it.
+struct Walk {
+    int pos, end, share;   // flat tiles
+    int first, cnt;        // flat index of sequence b's first tile, and how many it has
+    int b, nrt, nt, tlo;   // row tiles, token tiles, first token tile of the sequence
+    Kv8Seq s;
+    Seg seg;
+};
+
+// Tiles of a sequence; at least one per row tile, whatever its length.
 template <int RT>
-__device__ __forceinline__ long long seq_tiles(const AttendParams& p, const Kv8Seq& s, int& nrt, int& nt, int& tlo)
+__device__ __forceinline__ int seq_tiles(const AttendParams& p, const Kv8Seq& s, int& nrt, int& nt, int& tlo)
 {
-    nrt = (int)(((long long)s.n * p.G + RT - 1) / RT);
+    nrt = (s.n * p.G + RT - 1) / RT;
     const int have = (int)min((long long)max(s.len, 0), (long long)p.w.max_pages << p.w.lgP);
     const int low = s.len - s.n - p.window + 1;
     tlo = p.window && low > 0 ? low / kTile : 0;
     nt = max((have + kTile - 1) / kTile - tlo, 1);
-    return (long long)p.w.KV * nrt * nt;
+    return p.w.KV * nrt * nt;
 }
 
+// The segment at pos, which lies in sequence b or behind it.
 template <int RT>
 __device__ __forceinline__ void walk_enter(const AttendParams& p, Walk& k)
 {
-    // pos lies in sequence b or behind it
+    if (k.pos >= k.end) {
+        k.seg.t1 = k.seg.t0 = 0;
+        return;
+    }
+#pragma unroll 1
     while (k.pos >= k.first + k.cnt) {
         k.first += k.cnt;
         ++k.b;
         k.s = kv8_seq(p.w, k.b);
         k.cnt = seq_tiles<RT>(p, k.s, k.nrt, k.nt, k.tlo);
     }
-    const long long local = k.pos - k.first;
-    const long long item = local / k.nt;
-    const int t = (int)(local - item * k.nt);
-    k.h = (int)(item / k.nrt);
-    k.rt = (int)(item - (long long)k.h * k.nrt);
-    k.item0 = k.pos - t;
-    k.t0 = k.tlo + t;
-    k.t1 = (int)min((long long)k.tlo + k.nt, k.t0 + (k.end - k.pos));
+    const unsigned local = k.pos - k.first, item = local / k.nt, t = local - item * k.nt;
+    k.seg.h = item / k.nrt;
+    k.seg.rt = item - k.seg.h * k.nrt;
+    k.seg.row0 = k.s.row0, k.seg.n = k.s.n, k.seg.len = k.s.len;
+    k.seg.t0 = k.tlo + t;
+    k.seg.t1 = min(k.tlo + k.nt, k.seg.t0 + (k.end - k.pos));
+    const unsigned item0 = k.pos - t;
+    k.seg.c0 = item0 / k.share;
+    k.seg.c1 = (item0 + k.nt - 1) / k.share;
 }
 
-// The share of CTA c, and its first segment.  False: nothing to do.
+// The share of this CTA, and its first segment.  Lane l counts the sequences
+// 32 i + l.
 template <int RT>
-__device__ __forceinline__ bool walk_begin(const AttendParams& p, Walk& k)
+__device__ __forceinline__ void walk_begin(const AttendParams& p, Walk& k)
 {
     const int lane = threadIdx.x & 31;
-    long long total = 0;
-    int nrt, nt, tlo;
+    int total = 0, c0 = 0;  // c0: of the first 32 sequences, kept
+#pragma unroll 1
     for (int b0 = 0; b0 < p.w.B; b0 += 32) {
-        long long c = 0;
+        int c = 0, nrt, nt, tlo;
         if (b0 + lane < p.w.B) c = seq_tiles<RT>(p, kv8_seq(p.w, b0 + lane), nrt, nt, tlo);
-        for (int z = 16; z; z >>= 1) c += __shfl_xor_sync(~0u, c, z);
-        total += c;
+        if (b0 == 0) c0 = c;
+        total += __reduce_add_sync(~0u, c);
     }
-    k.share = max((total + gridDim.x - 1) / gridDim.x, (long long)p.min_share);
-    k.pos = k.share * blockIdx.x;
+    k.share = max((total + (int)gridDim.x - 1) / (int)gridDim.x, p.min_share);
+    k.pos = (int)min((long long)k.share * blockIdx.x, (long long)total);
     k.end = min(k.pos + k.share, total);
-    if (k.pos >= k.end) return false;
-    // the sequence that pos lies in
-    long long before = 0;
-    for (int b0 = 0;; b0 += 32) {
-        long long c = 0;
-        if (b0 + lane < p.w.B) c = seq_tiles<RT>(p, kv8_seq(p.w, b0 + lane), nrt, nt, tlo);
-        long long x = c;
+    k.first = k.cnt = 0;
+    k.b = -1;
+    // The 32 sequences that pos lies in, and the one of them.
+#pragma unroll 1
+    for (int b0 = 0; k.pos < k.end; b0 += 32) {
+        int c = c0, nrt, nt, tlo;
+        if (b0) c = b0 + lane < p.w.B ? seq_tiles<RT>(p, kv8_seq(p.w, b0 + lane), nrt, nt, tlo) : 0;
+        int x = c;
+#pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
-            const long long y = __shfl_up_sync(~0u, x, d);
+            const int y = __shfl_up_sync(~0u, x, d);
             if (lane >= d) x += y;
         }
-        const unsigned past = __ballot_sync(~0u, before + x > k.pos);
+        const unsigned past = __ballot_sync(~0u, k.first + x > k.pos);
         if (past) {
             const int l = __ffs(past) - 1;
-            k.b = b0 + l;
-            k.first = before + __shfl_sync(~0u, x - c, l);
+            k.b = b0 + l - 1;  // walk_enter reads the sequence itself
+            k.first += __shfl_sync(~0u, x - c, l);
             break;
         }
-        before += __shfl_sync(~0u, x, 31);
+        k.first += __shfl_sync(~0u, x, 31);
     }
-    k.s = kv8_seq(p.w, k.b);
-    k.cnt = seq_tiles<RT>(p, k.s, k.nrt, k.nt, k.tlo);
     walk_enter<RT>(p, k);
-    return true;
 }
 
 template <int RT>
-__device__ __forceinline__ bool walk_next(const AttendParams& p, Walk& k)
+__device__ __forceinline__ void walk_next(const AttendParams& p, Walk& k)
 {
-    k.pos += k.t1 - k.t0;
-    if (k.pos >= k.end) return false;
+    k.pos += k.seg.t1 - k.seg.t0;
     walk_enter<RT>(p, k);
-    return true;
 }
 
 // ------------------------------------------------------------- shared memory --
@@ -255,7 +268,7 @@ struct Shape {
 struct Bars {
     uint64_t kfull[kMaxStages], kempty[kMaxStages], vfull[kMaxStages], vempty[kMaxStages];
     uint64_t sfull[2], sempty[2], pfull[2], pempty[2], ofull[2], oempty[2], stfull[2], stempty[2];
-    uint64_t mfull[kMeta], qfull, pmax[2][2], jdone, jlast;
+    uint64_t mfull[kMeta], segfull[kMeta], qfull, pmax[2][2], jdone, jlast;
 };
 
 struct Meta {
@@ -265,20 +278,29 @@ struct Meta {
 };
 
 template <int RT>
-struct Small {
-    Bars bars;
-    Meta meta[kMeta];
+struct alignas(16) Small {
     float stat_max[2][4][RT], stat_sum[2][4][RT];  // per softmax warp: its page's maximum, its own sum of weights
-    float stat_vs[2][4];
     float wmax[2][4][RT];
     float qscale[2][RT];  // by the segment's parity
     int pos[2][RT];
-    float join[4][5][RT];  // per join warp: the factor of what was there, then of each page
+    float join[4][5][RT];      // per join warp: the factor of what was there, then of each page
+    float stat_vs[2][4];
+    Meta meta[kMeta];
+    Seg seg[kMeta];
+    Bars bars;
     uint32_t tmem;
     int abort;
     int last;
     int kfills[kMaxStages], vfills[kMaxStages];
 };
+
+template <int RT>
+__device__ __forceinline__ void store_rows(float* dst, const float (&x)[RT])
+{
+#pragma unroll
+    for (int r = 0; r < RT; r += 4)
+        *reinterpret_cast<float4*>(dst + r) = make_float4(x[r], x[r + 1], x[r + 2], x[r + 3]);
+}
 
 template <int DG, int RT, int HDW>
 __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const __grid_constant__ AttendParams p)
@@ -299,6 +321,7 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
     int* err = p.w.err;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int P = p.w.P, NP = kTile >> p.w.lgP;
+    auto over_g = [&](int f) { return (int)__umulhi((unsigned)f, p.inv_g) + (p.G == 1 ? f : 0); };
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < S; ++i) {
@@ -318,7 +341,10 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
             mbar_init(&br.stfull[i], 4);
             mbar_init(&br.stempty[i], 4);
         }
-        for (int i = 0; i < kMeta; ++i) mbar_init(&br.mfull[i], 1);
+        for (int i = 0; i < kMeta; ++i) {
+            mbar_init(&br.mfull[i], 1);
+            mbar_init(&br.segfull[i], 1);
+        }
         mbar_init(&br.qfull, 4);
         for (int i = 0; i < 4; ++i) mbar_init(&br.pmax[i >> 1][i & 1], P / 32);
         mbar_init(&br.jdone, 4);
@@ -338,68 +364,100 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
     const uint32_t tm_s = z.tmem, tm_o = z.tmem + p.nS * N;
     pdl_trigger();
     pdl_wait();
+    // The other warps' view of the walk: the next segment, once it is known.
+    // The ring cannot overrun: the copies are at most kMaxStages tiles ahead of
+    // the products, these 2 ahead of the softmax and that 2 ahead of the join.
+    int seg_at = 0;
+    auto next_seg = [&](Seg& k) -> bool {
+        const int i = seg_at % kMeta;
+        if (!warp_wait(&br.segfull[i], seg_at / kMeta & 1, err, abort)) return false;
+        k = z.seg[i];
+        ++seg_at;
+        return k.t1 > k.t0;
+    };
 
-    Walk k;
-    const bool any = walk_begin<RT>(p, k);
     uint64_t* last_bar = nullptr;  // of the product issued last
     int last_ph = 0;
-    if (any && warp == 8) {
+    if (warp == 8) {
         // ---------------------------------------------------------- copies --
+        // Page entries come in batches of up to 32 pages of one segment, one
+        // per lane, each fetched while the batch before it is copied.
         int st = 0, use = 0, mt = 0;
-        bool ok = true, more = true;
-        while (ok && more) {
-            const int pg_end = k.t1 * NP;
-            int unit = 0, nunit = 0, have = 0, nhave = 0;
-            float ks = 0, vs = 0, nks = 0, nvs = 0;
-            auto fetch = [&](int pg, int& u, int& hv, float& a, float& b) {
-                hv = 0, u = 0, a = 0.0f, b = 0.0f;
-                if (pg < pg_end && (long long)pg << p.w.lgP < k.s.len) {
-                    const int x = kv8_unit(p.w, k.s, pg, k.h);
-                    if (x >= 0) hv = 1, u = x, a = p.w.ks[x], b = p.w.vs[x];
-                }
-            };
-            int pg = k.t0 * NP;
-            fetch(pg + lane, nunit, nhave, nks, nvs);
-            int at = 32;  // lane of the tile's first page within the fetched 32
-            for (int t = k.t0; ok && t < k.t1; ++t, at += NP) {
-                if (at == 32) {
-                    unit = nunit, have = nhave, ks = nks, vs = nvs;
-                    pg += 32;
-                    fetch(pg + lane, nunit, nhave, nks, nvs);
-                    at = 0;
-                }
+        struct Batch {
+            int tiles, unit, have;
+            float ks, vs;
+        };
+        Walk k;
+        walk_begin<RT>(p, k);
+        auto publish = [&]() {
+            if (lane == 0) {
+                z.seg[seg_at % kMeta] = k.seg;
+                mbar_arrive(&br.segfull[seg_at % kMeta]);
+            }
+            ++seg_at;
+        };
+        publish();
+        int at_t = k.seg.t0;
+        auto fetch = [&]() -> Batch {
+            Batch f{0, 0, 0, 0.0f, 0.0f};
+            f.tiles = min(k.seg.t1 - at_t, 32 / NP);
+            if (f.tiles == 0) return f;
+            const int pg = at_t * NP + lane;
+            if (lane < f.tiles * NP && (long long)pg << p.w.lgP < k.s.len) {
+                const int x = kv8_unit(p.w, k.s, pg, k.seg.h);
+                if (x >= 0) f.have = 1, f.unit = x, f.ks = p.w.ks[x], f.vs = p.w.vs[x];
+            }
+            at_t += f.tiles;
+            if (at_t == k.seg.t1) {
+                walk_next<RT>(p, k);
+                publish();
+                at_t = k.seg.t0;
+            }
+            return f;
+        };
+        Batch nxt = fetch();
+        bool ok = true;
+        while (ok && nxt.tiles) {
+            const Batch cur = nxt;
+            nxt.tiles = -1;
+            for (int i = 0; ok && i < cur.tiles; ++i) {
+                const int at = i * NP, j = lane - at;
                 if (use > 0 && !(ok = warp_wait(&br.kempty[st], (use - 1) & 1, err, abort))) break;
                 const bool mine = lane >= at && lane < at + NP;
-                const int j = lane - at;
-                const unsigned valid = __ballot_sync(~0u, mine && have) >> at;
-                Meta& m = z.meta[mt];
-                if (mine) m.ks[j] = ks, m.vs[j] = vs;
                 if (lane == at) {
-                    m.valid = (int)valid;
                     z.kfills[st] += 1;
                     mbar_arrive_expect_tx(&br.kfull[st], kStage);
                 }
                 __syncwarp();
+                if (mine) tma_page(&p.kmap, ksm + st * kStage + j * P * HDW, cur.unit, &br.kfull[st]);
+                // The next batch's entries are under way while this tile's wait.
+                if (nxt.tiles < 0) nxt = fetch();
+                Meta& m = z.meta[mt];
+                const unsigned valid = __ballot_sync(~0u, mine && cur.have) >> at;
+                if (mine) m.ks[j] = cur.ks, m.vs[j] = cur.vs;
+                if (lane == at) m.valid = (int)valid;
+                __syncwarp();
                 if (lane == at) mbar_arrive(&br.mfull[mt]);
-                if (mine) tma_page(&p.kmap, ksm + st * kStage + j * P * HDW, unit, &br.kfull[st]);
                 if (use > 0 && !(ok = warp_wait(&br.vempty[st], (use - 1) & 1, err, abort))) break;
                 if (lane == at) {
                     z.vfills[st] += 1;
                     mbar_arrive_expect_tx(&br.vfull[st], kStage);
                 }
                 __syncwarp();
-                if (mine) tma_page(&p.vmap, vsm + st * kStage + j * P * HDW, unit, &br.vfull[st]);
+                if (mine) tma_page(&p.vmap, vsm + st * kStage + j * P * HDW, cur.unit, &br.vfull[st]);
                 if (++st == S) st = 0, ++use;
                 if (++mt == kMeta) mt = 0;
             }
-            more = ok && walk_next<RT>(p, k);
         }
-    } else if (any && warp == 9) {
+    } else if (warp == 9) {
         // ------------------------------------------------------------ MMAs --
         const uint32_t idS = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | (8u << 24);
         const uint32_t idO = (2u << 4) | (1u << 7) | (1u << 15) | ((uint32_t)(N >> 3) << 17) | (8u << 24);
         int kst = 0, kuse = 0, vst = 0, vuse = 0, sb = 0, su = 0, pb = 0, pu = 0, ob = 0, ou = 0, seg = 0;
-        const uint32_t qa = sptr(qsm), ka = sptr(ksm), va = sptr(vsm), pa = sptr(psm);
+        // An address moves a descriptor by its sixteenth.
+        const uint64_t qd = desc_of(sptr(qsm), 8 * HDW, kSw), kd = desc_of(sptr(ksm), 8 * HDW, kSw);
+        const uint64_t vd = desc_of(sptr(vsm), 8 * HDW, kSw), pd = desc_of(sptr(psm), 1024, 2u);
+        const int lg_per = p.w.lgP - 5, first_of = (1 << lg_per) - 1;
         auto issue_s = [&](bool fresh) -> bool {
             if (fresh && !warp_wait(&br.qfull, seg++ & 1, err, abort)) return false;
             if (!warp_wait(&br.kfull[kst], kuse & 1, err, abort)) return false;
@@ -408,8 +466,7 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
             if (elect()) {
 #pragma unroll
                 for (int i = 0; i < HDW / 32; ++i)
-                    mma_i8(tm_s + sb * N, desc_of(ka + kst * kStage + 32 * i, 8 * HDW, kSw),
-                           desc_of(qa + 32 * i, 8 * HDW, kSw), idS, i > 0);
+                    mma_i8(tm_s + sb * N, kd + (uint32_t)(kst * (kStage / 16) + 2 * i), qd + 2 * i, idS, i > 0);
                 mma_commit(&br.sfull[sb]);
                 mma_commit(&br.kempty[kst]);
             }
@@ -425,11 +482,10 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
             if (ou > 0 && !warp_wait(&br.oempty[ob], (ou - 1) & 1, err, abort)) return false;
             fence_after();
             if (elect()) {
-                const int per = P / 32;
 #pragma unroll
                 for (int i = 0; i < kTile / 32; ++i)  // 32 tokens each
-                    mma_i8(tm_o + (ob * NP + i / per) * N, desc_of(va + vst * kStage + 32 * HDW * i, 8 * HDW, kSw),
-                           desc_of(pa + pb * kPBytes + 32 * i, 1024, 2u), idO, i % per > 0);
+                    mma_i8(tm_o + (ob * NP + (i >> lg_per)) * N, vd + (uint32_t)(vst * (kStage / 16) + 2 * HDW * i),
+                           pd + (uint32_t)(pb * (kPBytes / 16) + 2 * i), idO, (i & first_of) > 0);
                 mma_commit(&br.ofull[ob]);
                 mma_commit(&br.pempty[pb]);
                 mma_commit(&br.vempty[vst]);
@@ -441,40 +497,53 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
             if (++ob == p.nO) ob = 0, ++ou;
             return true;
         };
-        bool ok = issue_s(true);
-        while (ok) {
-            for (int t = k.t0; ok && t < k.t1; ++t) {
-                if (t + 1 < k.t1) ok = issue_s(false);
+        Seg k;
+        bool more = next_seg(k), ok = !more || issue_s(true);
+        while (ok && more) {
+            const int t1 = k.t1;
+            for (int t = k.t0; ok && t < t1; ++t) {
+                if (t + 1 < t1) ok = issue_s(false);
                 ok = ok && issue_o();
             }
-            if (!ok || !walk_next<RT>(p, k)) break;
+            if (!ok || !(more = next_seg(k))) break;
             ok = issue_s(true);
         }
-    } else if (any && warp < 4) {
+    } else if (warp < 4) {
         // --------------------------------------------------------- softmax --
         const int tid = threadIdx.x, page = tid >> p.w.lgP;
         int sb = 0, su = 0, pb = 0, pu = 0, mt = 0, mu = 0, seg = 0;
         const uint32_t tm = tm_s + ((uint32_t)warp << 21);
         constexpr float kQMax = DG == 3 ? 8323072.0f : 32512.0f;  // 127 * 256^(DG-1)
-        bool ok = true, more = true;
+        // Query rows warp, warp + 4, ... of a row tile; lane l has 4 elements.
+        constexpr int kRows = RT / 4;
+        auto load_q = [&](const Seg& k, float (&x)[kRows][4]) {
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) {
+                const int f = k.rt * RT + 4 * i + warp, qi = over_g(f), g = f - qi * p.G, e = lane * 4;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[i][j] = 0.0f;
+                if (qi >= k.n || e >= p.w.hd) continue;
+                const size_t off = (size_t)(k.row0 + qi) * p.ldq + (size_t)(k.h * p.G + g) * p.w.hd + e;
+                if (p.type == QUANTR_TYPE_F32)
+                    load4<float>(static_cast<const float*>(p.q) + off, p.vec, x[i]);
+                else if (p.type == T_F16)
+                    load4<__half>(static_cast<const __half*>(p.q) + off, p.vec, x[i]);
+                else
+                    load4<__nv_bfloat16>(static_cast<const __nv_bfloat16*>(p.q) + off, p.vec, x[i]);
+            }
+        };
+        float qx[kRows][4];
+        Seg k;
+        bool ok = true, more = next_seg(k);
+        if (more) load_q(k, qx);
         while (ok && more) {
             // The row tile's query rows as digits.  Its last product has read
             // the old ones (its scores have arrived).
-            const int base_pos = k.s.len - k.s.n, sg = seg & 1;
-            for (int r = warp; r < RT; r += 4) {
-                const int f = k.rt * RT + r, qi = f / p.G, g = f - qi * p.G;
-                const bool live = qi < k.s.n;
-                float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                const int e = lane * 4;
-                if (live && e < p.w.hd) {
-                    const size_t off = (size_t)(k.s.row0 + qi) * p.ldq + (size_t)(k.h * p.G + g) * p.w.hd + e;
-                    if (p.type == QUANTR_TYPE_F32)
-                        load4<float>(static_cast<const float*>(p.q) + off, false, x);
-                    else if (p.type == T_F16)
-                        load4<__half>(static_cast<const __half*>(p.q) + off, false, x);
-                    else
-                        load4<__nv_bfloat16>(static_cast<const __nv_bfloat16*>(p.q) + off, false, x);
-                }
+            const int base_pos = k.len - k.n, sg = seg & 1;
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) {
+                const int r = 4 * i + warp, e = lane * 4;
+                const float* x = qx[i];
                 const float top = warp_max_nan(max_nan(max_nan(fabsf(x[0]), fabsf(x[1])), max_nan(fabsf(x[2]), fabsf(x[3]))));
                 const bool fine = top <= 3.402823466e38f;
                 // The largest power of two that keeps the row's largest element
@@ -488,12 +557,12 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
                 }
                 uint32_t dig[3] = {0, 0, 0};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    int v = fine ? __float2int_rn(x[i] * inv) : 0;
+                for (int j = 0; j < 4; ++j) {
+                    int v = fine ? __float2int_rn(x[j] * inv) : 0;
 #pragma unroll
                     for (int d = DG - 1; d >= 0; --d) {
                         const int lo = (int)(int8_t)v;
-                        dig[d] |= (uint32_t)(lo & 255) << (8 * i);
+                        dig[d] |= (uint32_t)(lo & 255) << (8 * j);
                         v = (v - lo) >> 8;
                     }
                 }
@@ -507,7 +576,7 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
                 }
                 if (lane == 0) {
                     z.qscale[sg][r] = fine ? step * p.scale2 : __int_as_float(0x7fffffff);
-                    z.pos[sg][r] = base_pos + qi;
+                    z.pos[sg][r] = base_pos + over_g(k.rt * RT + r);
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -516,7 +585,12 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
             if (!(ok = warp_wait(&br.qfull, seg++ & 1, err, abort))) break;
             const int pos_lo = z.pos[sg][0], pos_hi = z.pos[sg][RT - 1];
 
-            for (int t = k.t0; t < k.t1; ++t) {
+            const int t0 = k.t0, t1 = k.t1;
+            for (int t = t0; t < t1; ++t) {
+                if (t + 1 == t1) {  // the next row tile's rows come during the last tile
+                    more = next_seg(k);
+                    if (more) load_q(k, qx);
+                }
                 ok = warp_wait(&br.mfull[mt], mu & 1, err, abort) && warp_wait(&br.sfull[sb], su & 1, err, abort);
                 if (!ok) break;
                 const Meta& m = z.meta[mt];
@@ -562,14 +636,17 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
                 if (P > 32) {  // the page spans several warps
                     const int w0 = P == 64 ? warp & 2 : 0, wn = P / 32;
                     if (lane == 0) {
-#pragma unroll
-                        for (int r = 0; r < RT; ++r) z.wmax[pb][warp][r] = mx[r];
+                        store_rows<RT>(z.wmax[pb][warp], mx);
                         mbar_arrive(&br.pmax[pb][w0 >> 1]);
                     }
                     if (!(ok = warp_wait(&br.pmax[pb][w0 >> 1], pu & 1, err, abort))) break;
                     for (int w = w0; w < w0 + wn; ++w) {
 #pragma unroll
-                        for (int r = 0; r < RT; ++r) mx[r] = max_nan(mx[r], z.wmax[pb][w][r]);
+                        for (int r = 0; r < RT; r += 4) {
+                            const float4 v = *reinterpret_cast<const float4*>(&z.wmax[pb][w][r]);
+                            mx[r] = max_nan(mx[r], v.x), mx[r + 1] = max_nan(mx[r + 1], v.y);
+                            mx[r + 2] = max_nan(mx[r + 2], v.z), mx[r + 3] = max_nan(mx[r + 3], v.w);
+                        }
                     }
                 }
                 if (pu > 0) {
@@ -577,6 +654,7 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
                          warp_wait(&br.stempty[pb], (pu - 1) & 1, err, abort);
                     if (!ok) break;
                 }
+                float sum[RT];
                 uint8_t* pt = psm + pb * kPBytes + (tid & 15);
 #pragma unroll
                 for (int r = 0; r < RT; ++r) {
@@ -596,11 +674,12 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
                         pt[(n0)*128 + sw * 16] = (uint8_t)(d >> 8);
                         pt[(n0 + RT) * 128 + ((tid >> 4) ^ ((n0 + RT) & 7)) * 16] = (uint8_t)d;
                     }
-                    const uint32_t sum = __reduce_add_sync(~0u, u - 0x3f800000u);
-                    if (lane == 0) {
-                        z.stat_sum[pb][warp][r] = (float)sum * (1.0f / 8388608.0f);
-                        z.stat_max[pb][warp][r] = mx[r];
-                    }
+                    // u - 0x3f800000 per lane
+                    sum[r] = (float)(__reduce_add_sync(~0u, u) - 32u * 0x3f800000u) * (1.0f / 8388608.0f);
+                }
+                if (lane == 0) {
+                    store_rows<RT>(z.stat_sum[pb][warp], sum);
+                    store_rows<RT>(z.stat_max[pb][warp], mx);
                 }
                 if (tid < NP) z.stat_vs[pb][tid] = m.vs[tid];
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -613,16 +692,55 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
                 if (++pb == 2) pb = 0, ++pu;
                 if (++mt == kMeta) mt = 0, ++mu;
             }
-            more = ok && walk_next<RT>(p, k);
         }
-    } else if (any && warp < 8) {
+    } else if (warp < 8) {
         // ------------------------------------------------------------ join --
         const int tid = threadIdx.x - 128, w4 = warp - 4;
         const uint32_t tm = tm_o + ((uint32_t)w4 << 21);
-        int sb = 0, su = 0, ob = 0, ou = 0, parts = 0;
+        int sb = 0, su = 0, ob = 0, ou = 0, meets = 0;
         bool ok = true, more = true;
         constexpr float kUnit = DG == 3 ? 1.0f / 8388608.0f : 1.0f / 65536.0f;
-        while (ok && more) {
+        constexpr size_t kPart = RT * 130;
+        const int me = blockIdx.x;
+        // Offsets of the row tile's rows, in lane r that of row r (-1: no such
+        // row); element `e` of a row from there.
+        auto row_of = [&](const Seg& k, long long& off, long long& lse) {
+            const int f = k.rt * RT + (lane & (RT - 1)), qi = over_g(f), hq = k.h * p.G + f - qi * p.G;
+            const long long row = k.row0 + qi;
+            off = qi < k.n ? row * p.ldo + (long long)hq * p.w.hd : -1;
+            lse = row * p.H + hq;
+        };
+        auto put = [&](long long off, float v) {
+            if (p.type == QUANTR_TYPE_F32) static_cast<float*>(p.out)[off] = v;
+            else if (p.type == T_F16) static_cast<__half*>(p.out)[off] = __float2half_rn(v);
+            else static_cast<__nv_bfloat16*>(p.out)[off] = __float2bfloat16_rn(v);
+        };
+        auto lse_of = [&](float m, float l) {
+            return m == -INFINITY ? m : (m + log2f(l) + (DG == 3 ? 0.0f : 2.2013990e-5f)) * 0.693147180559945f;
+        };
+        // Counts this CTA in; true in all join threads if it is the last of n,
+        // and then the others' parts can be read.
+        auto last_of = [&](int* counter, int n, bool& last) -> bool {
+            __threadfence();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&br.jdone);
+            if (tid == 0 && mbar_wait_bounded(&br.jdone, meets & 1, err, abort)) {
+                z.last = atomicAdd(counter, 1) == n - 1;
+                if (z.last) *counter = 0;
+                __threadfence();
+                mbar_arrive(&br.jlast);
+            }
+            __syncwarp();
+            if (!warp_wait(&br.jlast, meets++ & 1, err, abort)) return false;
+            last = z.last;
+            return true;
+        };
+        // Row tiles that this CTA shares with others: the one it came into and
+        // the one it leaves.
+        Seg shared0{}, shared1{};
+        int n_shared = 0;
+        Seg k;
+        while (ok && next_seg(k)) {
             float o[RT];
 #pragma unroll
             for (int r = 0; r < RT; ++r) o[r] = 0.0f;
@@ -686,78 +804,89 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
                 if (++ob == p.nO) ob = 0, ++ou;
             }
             if (!ok) break;
-            // Whole row tile: write it.  Part of one: leave it in the
-            // workspace, and join all parts if this is the last to come.
-            const long long item1 = k.item0 + k.nt;
-            const int c0 = (int)(k.item0 / k.share), c1 = (int)((item1 - 1) / k.share);
-            float l[RT], mrow[RT];
-#pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                l[r] = __shfl_sync(~0u, l_run, r);
-                mrow[r] = __shfl_sync(~0u, m_run, r);
-            }
-            bool write = true;
-            if (c0 != c1) {
-                constexpr int kPart = RT * 130;
-                float* mine = p.part + (size_t)(2 * blockIdx.x + ((int)blockIdx.x == c0 ? 1 : 0)) * kPart;
-#pragma unroll
-                for (int r = 0; r < RT; ++r) mine[r * 128 + tid] = o[r];
-                if (w4 == 0 && lane < RT) mine[RT * 128 + lane] = m_run, mine[RT * 129 + lane] = l_run;
-                __threadfence();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&br.jdone);
-                if (tid == 0 && mbar_wait_bounded(&br.jdone, parts & 1, err, abort)) {
-                    const int n = atomicAdd(p.counters + c0, 1);
-                    z.last = n == c1 - c0;
-                    if (z.last) p.counters[c0] = 0;
-                    __threadfence();
-                    mbar_arrive(&br.jlast);
-                }
-                __syncwarp();
-                if (!(ok = warp_wait(&br.jlast, parts++ & 1, err, abort))) break;
-                write = z.last;
-                if (write) {
-                    float mall[RT];
-#pragma unroll
-                    for (int r = 0; r < RT; ++r) mall[r] = -INFINITY, l[r] = 0.0f, o[r] = 0.0f;
-                    for (int c = c0; c <= c1; ++c) {
-                        const float* part = p.part + (size_t)(2 * c + (c == c0 ? 1 : 0)) * kPart;
-#pragma unroll
-                        for (int r = 0; r < RT; ++r) {
-                            const float mp = __ldcg(part + RT * 128 + r), lp = __ldcg(part + RT * 129 + r);
-                            const float mn = max_nan(mall[r], mp), ref = mn == -INFINITY ? 0.0f : mn;
-                            const float a = ex2(mall[r] - ref), f = ex2(mp - ref);
-                            l[r] = fmaf(lp, f, l[r] * a);
-                            o[r] = fmaf(__ldcg(part + r * 128 + tid), f, o[r] * a);
-                            mall[r] = mn;
-                        }
-                    }
-#pragma unroll
-                    for (int r = 0; r < RT; ++r) mrow[r] = mall[r];
-                }
-            }
-            if (write) {
+            if (k.c0 == k.c1) {
+                long long off, at;
+                row_of(k, off, at);
+                const float inv = m_run == -INFINITY ? 0.0f : 1.0f / l_run;  // nothing seen: o is 0
+                if (p.lse && w4 == 0 && lane < RT && off >= 0) p.lse[at] = lse_of(m_run, l_run);
 #pragma unroll
                 for (int r = 0; r < RT; ++r) {
-                    const int f = k.rt * RT + r, qi = f / p.G, g = f - qi * p.G;
-                    if (qi >= k.s.n) continue;
-                    const size_t row = (size_t)k.s.row0 + qi;
-                    const int hq = k.h * p.G + g;
-                    const bool none = mrow[r] == -INFINITY;
-                    if (tid < p.w.hd) {
-                        const float v = none ? 0.0f : o[r] / l[r];
-                        const size_t off = row * p.ldo + (size_t)hq * p.w.hd + tid;
-                        if (p.type == QUANTR_TYPE_F32) static_cast<float*>(p.out)[off] = v;
-                        else if (p.type == T_F16) static_cast<__half*>(p.out)[off] = __float2half_rn(v);
-                        else static_cast<__nv_bfloat16*>(p.out)[off] = __float2bfloat16_rn(v);
-                    }
-                    if (p.lse && tid == 0)
-                        p.lse[row * p.H + hq] =
-                            none ? -INFINITY
-                                 : (mrow[r] + log2f(l[r]) + (DG == 3 ? 0.0f : 2.2013990e-5f)) * 0.693147180559945f;
+                    const long long to = __shfl_sync(~0u, off, r);
+                    const float v = o[r] * __shfl_sync(~0u, inv, r);
+                    if (to >= 0 && tid < p.w.hd) put(to + tid, v);
                 }
+            } else {
+                // A part: o[RT][128], m[RT], l[RT].
+                float* part = p.part + (2 * (size_t)me + (me == k.c0 ? 1 : 0)) * kPart;
+#pragma unroll
+                for (int r = 0; r < RT; ++r) part[r * 128 + tid] = o[r];
+                if (w4 == 0 && lane < RT) part[RT * 128 + lane] = m_run, part[RT * 129 + lane] = l_run;
+                if (n_shared++) shared1 = k;
+                else shared0 = k;
             }
-            more = walk_next<RT>(p, k);
+        }
+        // Joins the n <= 32 parts at base, base + stride, ... (the first of them
+        // one part further when `shift`), row by row: warp w4 takes the rows w4,
+        // w4 + 4, ...; lane i weighs part i, and has 4 of the row's elements.
+        // To another part, or (null) to the output.
+        auto join_parts = [&](const float* base, int n, size_t stride, bool shift, float* to, const Seg& k) {
+            long long off, at;
+            row_of(k, off, at);
+#pragma unroll 1
+            for (int r = w4; r < RT; r += 4) {
+                const float* mine = base + lane * stride + (shift && lane == 0 ? kPart : 0) + RT * 128 + r;
+                float m = -INFINITY, l = 0.0f;
+                if (lane < n) m = __ldcg(mine), l = __ldcg(mine + RT);
+                const float top = warp_max_nan(m), f = ex2(m - (top == -INFINITY ? 0.0f : top));
+                l *= f;
+#pragma unroll
+                for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(~0u, l, d);
+                float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+                for (int i = 0; i < n; ++i) {
+                    const float4 v = __ldcg(reinterpret_cast<const float4*>(
+                        base + i * stride + (shift && i == 0 ? kPart : 0) + r * 128 + lane * 4));
+                    const float g = __shfl_sync(~0u, f, i);
+                    o.x = fmaf(v.x, g, o.x), o.y = fmaf(v.y, g, o.y), o.z = fmaf(v.z, g, o.z), o.w = fmaf(v.w, g, o.w);
+                }
+                if (to) {
+                    *reinterpret_cast<float4*>(to + r * 128 + lane * 4) = o;
+                    if (lane == 0) to[RT * 128 + r] = top, to[RT * 129 + r] = l;
+                    continue;
+                }
+                const long long row = __shfl_sync(~0u, off, r), lse = __shfl_sync(~0u, at, r);
+                if (row < 0) continue;
+                const float inv = 1.0f / l;
+                const float v[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+                if (lane * 4 < p.w.hd) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) put(row + lane * 4 + j, top == -INFINITY ? 0.0f : v[j]);
+                }
+                if (p.lse && lane == 0) p.lse[lse] = lse_of(top, l);
+            }
+        };
+        // Shared row tiles: whoever comes last joins them, in token order.
+#pragma unroll 1
+        for (int i = 0; ok && i < n_shared; ++i) {
+            const Seg q = i ? shared1 : shared0;
+            bool last = false;
+            int n = q.c1 - q.c0 + 1;
+            const int g0 = q.c0 + (me - q.c0) / kGroup * kGroup;
+            const bool grouped = n > kChunk;
+            int* counter = p.counters + (grouped ? g0 : kMaxCtas + q.c0);
+            const float* base = p.part + 2 * (size_t)(grouped ? g0 : q.c0) * kPart;
+            size_t stride = 2 * kPart;
+            int gn = grouped ? min(kGroup, q.c1 - g0 + 1) : n;
+#pragma unroll 1
+            for (int level = grouped ? 0 : 1; level < 2; ++level) {
+                if (!(ok = last_of(counter, gn, last)) || !last) break;
+                const bool shift = level || g0 == q.c0;
+                join_parts(base, gn, stride, shift, level ? nullptr : const_cast<float*>(base) + (shift ? kPart : 0), q);
+                counter = p.counters + kMaxCtas + q.c0;
+                base = p.part + 2 * (size_t)q.c0 * kPart;
+                stride = 2 * kPart * kGroup;
+                gn = (n + kGroup - 1) / kGroup;
+            }
         }
     }
 
@@ -898,14 +1027,22 @@ int quantr_kv8_attend_dev(void* out, long long ldo, const void* q, long long ldq
     if (!workspace || ((uintptr_t)workspace & 255) ||
         workspace_bytes < quantr_kv8_attend_workspace_bytes(pool, batch, n_heads, max_len))
         return QUANTR_ERR_WORKSPACE;
+    const int rt = pick_rt(batch, n_heads / pool->n_kv_heads);
+    {  // flat tile numbers and f * G (above) are 32-bit
+        const double G = n_heads / pool->n_kv_heads, rows = (double)batch->max_rows * G + rt;
+        const double tiles = (double)tables->max_pages * pool->page_tokens / kTile + 1;
+        if (rows * G >= 4294967296.0 || (double)batch->B * pool->n_kv_heads * (rows / rt + 1) * tiles >= 2147483648.0)
+            return QUANTR_ERR_TOO_LARGE;
+    }
     AttendParams p{};
     p.w = kv8_view(pool, tables, batch, layer);
     p.q = q, p.out = out, p.lse = lse, p.ldq = ldq, p.ldo = ldo, p.type = type;
+    p.vec = aligned4(q, ldq, type == QUANTR_TYPE_F32 ? 4 : 2);
     p.H = n_heads, p.G = n_heads / pool->n_kv_heads, p.window = window;
+    p.inv_g = p.G == 1 ? 0 : (unsigned)(((1ull << 32) + p.G - 1) / p.G);
     p.scale2 = (float)((double)scale * 1.4426950408889634);
     LaunchCfg c;
     c.stream = (cudaStream_t)stream;
-    const int rt = pick_rt(batch, p.G);
     cudaError_t e;
     if (type == QUANTR_TYPE_F32)
         e = pool->head_dim <= 64 ? run_rt<3, 64>(rt, p, pool, workspace, c) : run_rt<3, 128>(rt, p, pool, workspace, c);
