@@ -46,6 +46,7 @@ constexpr int kMaxStages = 6;
 constexpr int kChunk = 32;     // parts of a row tile joined at once
 constexpr int kGroup = 16;     // more of them than kChunk are joined in groups first
 constexpr int kMaxCtas = 512;
+constexpr int kSlack = 5;      // tiles that sharing out by row tiles may cost the longest CTA
 
 struct AttendParams {
     CUtensorMap kmap, vmap;
@@ -54,12 +55,11 @@ struct AttendParams {
     void* out;
     float* lse;
     long long ldq, ldo;
-    uint32_t type;
     int H, G, window;
     unsigned inv_g;  // ceil(2^32 / G): f / G = umulhi(f, inv_g) for f * G < 2^32 (G = 1 apart)
     float scale2;  // scale * log2(e)
     int vec;       // query rows allow aligned loads of four
-    int stages, nS, nO, tmem_cols, min_share;
+    int stages, nS, nO, tmem_cols;
     int* counters;  // [2][kMaxCtas] by a row tile's (a group's) first CTA, zero between calls
     float* part;    // 2 per CTA: o [RT][128], m [RT], l [RT]
 };
@@ -208,30 +208,62 @@ __device__ __forceinline__ void walk_enter(const AttendParams& p, Walk& k)
     k.seg.c1 = (item0 + k.nt - 1) / k.share;
 }
 
-// The share of this CTA, and its first segment.  Lane l counts the sequences
-// 32 i + l.
+// This CTA's part of the work and its first segment.  Two ways to share it out:
+//   by row tiles, where there are no more of them than CTAs and their lengths
+//   differ little: a row tile has `per` CTAs, each with one run of its tiles
+//   (at least sqrt(nt/6): a part costs the join about a sixth of a tile);
+//   by tiles, else: equal runs of the flat list of all tiles.
+// Lane l looks at the sequences 32 i + l.
 template <int RT>
 __device__ __forceinline__ void walk_begin(const AttendParams& p, Walk& k)
 {
-    const int lane = threadIdx.x & 31;
-    int total = 0, c0 = 0;  // c0: of the first 32 sequences, kept
+    const int lane = threadIdx.x & 31, ctas = gridDim.x, me = blockIdx.x;
+    int tiles = 0, items = 0, longest = 0;
+    constexpr int kKept = 4;
+    int nts[kKept], its[kKept];  // of the first 128 sequences, read at once and kept
+    auto look = [&](int b0, int& nt, int& it) {
+        int nrt, tlo;
+        nt = it = 0;
+        if (b0 + lane < p.w.B) {
+            const Kv8Seq s = kv8_seq(p.w, b0 + lane);
+            const int all = seq_tiles<RT>(p, s, nrt, nt, tlo);
+            it = all ? p.w.KV * nrt : 0;
+        }
+    };
+    auto add = [&](int nt, int it) {
+        tiles += nt * it;
+        items += it;
+        longest = max(longest, it ? nt : 0);
+    };
+#pragma unroll
+    for (int i = 0; i < kKept; ++i) look(32 * i, nts[i], its[i]);
+#pragma unroll
+    for (int i = 0; i < kKept; ++i) add(nts[i], its[i]);
 #pragma unroll 1
-    for (int b0 = 0; b0 < p.w.B; b0 += 32) {
-        int c = 0, nrt, nt, tlo;
-        if (b0 + lane < p.w.B) c = seq_tiles<RT>(p, kv8_seq(p.w, b0 + lane), nrt, nt, tlo);
-        if (b0 == 0) c0 = c;
-        total += __reduce_add_sync(~0u, c);
+    for (int b0 = 32 * kKept; b0 < p.w.B; b0 += 32) {
+        int nt, it;
+        look(b0, nt, it);
+        add(nt, it);
     }
-    k.share = max((total + (int)gridDim.x - 1) / (int)gridDim.x, p.min_share);
-    k.pos = (int)min((long long)k.share * blockIdx.x, (long long)total);
-    k.end = min(k.pos + k.share, total);
+    tiles = __reduce_add_sync(~0u, tiles);
+    items = __reduce_add_sync(~0u, items);
+    longest = __reduce_max_sync(~0u, longest);
+    k.share = (tiles + ctas - 1) / max(ctas, 1);
+    const int per = items > 0 ? ctas / items : 0;
+    const bool by_items = per > 0 && (longest + per - 1) / per <= k.share + kSlack;
+    k.pos = by_items ? me / per : min((int)min((long long)k.share * me, 0x7fffffffll), tiles);
+    k.end = by_items ? items : min(k.pos + k.share, tiles);
     k.first = k.cnt = 0;
     k.b = -1;
     // The 32 sequences that pos lies in, and the one of them.
 #pragma unroll 1
     for (int b0 = 0; k.pos < k.end; b0 += 32) {
-        int c = c0, nrt, nt, tlo;
-        if (b0) c = b0 + lane < p.w.B ? seq_tiles<RT>(p, kv8_seq(p.w, b0 + lane), nrt, nt, tlo) : 0;
+        int nt = nts[0], it = its[0];
+#pragma unroll
+        for (int i = 1; i < kKept; ++i)
+            if (b0 == 32 * i) nt = nts[i], it = its[i];
+        if (b0 >= 32 * kKept) look(b0, nt, it);
+        const int c = by_items ? it : nt * it;
         int x = c;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -247,6 +279,25 @@ __device__ __forceinline__ void walk_begin(const AttendParams& p, Walk& k)
         }
         k.first += __shfl_sync(~0u, x, 31);
     }
+    if (by_items && k.pos < k.end) {
+        // Row tile `pos` as a list of its own: walk_enter sees the tiles of the
+        // part, no others.
+        const int part = me - k.pos * per;
+        ++k.b;
+        k.s = kv8_seq(p.w, k.b);
+        seq_tiles<RT>(p, k.s, k.nrt, k.nt, k.tlo);
+        const int item = k.pos - k.first;
+        const int run = max((k.nt + per - 1) / per, (int)ceilf(sqrtf((float)k.nt * (1.0f / 6.0f))));
+        k.seg.h = item / k.nrt;
+        k.seg.rt = item - k.seg.h * k.nrt;
+        k.seg.row0 = k.s.row0, k.seg.n = k.s.n, k.seg.len = k.s.len;
+        k.seg.t0 = min(part * run, k.nt) + k.tlo;
+        k.seg.t1 = min(part * run + run, k.nt) + k.tlo;
+        k.seg.c0 = k.pos * per;
+        k.seg.c1 = k.seg.c0 + (k.nt + run - 1) / run - 1;
+        k.pos = k.end = 0;  // and no more after it
+        return;
+    }
     walk_enter<RT>(p, k);
 }
 
@@ -258,6 +309,10 @@ __device__ __forceinline__ void walk_next(const AttendParams& p, Walk& k)
 }
 
 // ------------------------------------------------------------- shared memory --
+
+// Digits of queries and weights: three for fp32, two for 16-bit types.
+template <typename T>
+constexpr int digits = sizeof(T) == 4 ? 3 : 2;
 
 template <int DG, int RT>
 struct Shape {
@@ -279,7 +334,8 @@ struct Meta {
 
 template <int RT>
 struct alignas(16) Small {
-    float stat_max[2][4][RT], stat_sum[2][4][RT];  // per softmax warp: its page's maximum, its own sum of weights
+    float stat_max[2][4][RT];  // per softmax warp: its page's maximum
+    float stat_sum[2][4][RT];  // and the sum of its 32 (bits of 1 + weight), an unsigned integer
     float wmax[2][4][RT];
     float qscale[2][RT];  // by the segment's parity
     int pos[2][RT];
@@ -302,9 +358,32 @@ __device__ __forceinline__ void store_rows(float* dst, const float (&x)[RT])
         *reinterpret_cast<float4*>(dst + r) = make_float4(x[r], x[r + 1], x[r + 2], x[r + 3]);
 }
 
-template <int DG, int RT, int HDW>
+template <int N>
+__device__ __forceinline__ void load_rows(const float* src, float (&x)[N])
+{
+#pragma unroll
+    for (int r = 0; r < N; r += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(src + r);
+        x[r] = v.x, x[r + 1] = v.y, x[r + 2] = v.z, x[r + 3] = v.w;
+    }
+}
+
+// Value of column r's digits.  A digit's sum over 128 products is below 2^22 in
+// magnitude, so two of them make one int32.  Conversions are slow here (they
+// share a quarter-rate pipe with ex2): the third digit takes 1.5 * 2^23 in its
+// integer, which is a float's bit pattern.
+template <int DG, int C>
+__device__ __forceinline__ float digits_value(const int (&c)[DG][C], int r)
+{
+    const float hi = (float)(c[0][r] * 256 + c[1][r]);
+    if constexpr (DG == 2) return hi;
+    else return fmaf(hi, 256.0f, __int_as_float(0x4b400000 + c[2][r]) - 12582912.0f);
+}
+
+template <typename T, int RT, int HDW>
 __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const __grid_constant__ AttendParams p)
 {
+    constexpr int DG = digits<T>;
     constexpr int N = Shape<DG, RT>::N;
     constexpr uint32_t kStage = kTile * HDW, kPBytes = Shape<DG, RT>::kPBytes;
     constexpr uint32_t kSw = HDW == 128 ? 2u : 4u;  // 128- or 64-byte swizzle
@@ -320,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
     volatile int* abort = &z.abort;
     int* err = p.w.err;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int P = p.w.P, NP = kTile >> p.w.lgP;
+    const int P = p.w.P, lgP = p.w.lgP, NP = kTile >> lgP;
     auto over_g = [&](int f) { return (int)__umulhi((unsigned)f, p.inv_g) + (p.G == 1 ? f : 0); };
 
     if (threadIdx.x == 0) {
@@ -346,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
             mbar_init(&br.segfull[i], 1);
         }
         mbar_init(&br.qfull, 4);
-        for (int i = 0; i < 4; ++i) mbar_init(&br.pmax[i >> 1][i & 1], P / 32);
+        for (int i = 0; i < 4; ++i) mbar_init(&br.pmax[i >> 1][i & 1], 1 << (lgP - 5));
         mbar_init(&br.jdone, 4);
         mbar_init(&br.jlast, 1);
         z.abort = 0;
@@ -457,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
         // An address moves a descriptor by its sixteenth.
         const uint64_t qd = desc_of(sptr(qsm), 8 * HDW, kSw), kd = desc_of(sptr(ksm), 8 * HDW, kSw);
         const uint64_t vd = desc_of(sptr(vsm), 8 * HDW, kSw), pd = desc_of(sptr(psm), 1024, 2u);
-        const int lg_per = p.w.lgP - 5, first_of = (1 << lg_per) - 1;
+        const int lg_per = lgP - 5, first_of = (1 << lg_per) - 1;
         auto issue_s = [&](bool fresh) -> bool {
             if (fresh && !warp_wait(&br.qfull, seg++ & 1, err, abort)) return false;
             if (!warp_wait(&br.kfull[kst], kuse & 1, err, abort)) return false;
@@ -524,12 +603,7 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
                 for (int j = 0; j < 4; ++j) x[i][j] = 0.0f;
                 if (qi >= k.n || e >= p.w.hd) continue;
                 const size_t off = (size_t)(k.row0 + qi) * p.ldq + (size_t)(k.h * p.G + g) * p.w.hd + e;
-                if (p.type == QUANTR_TYPE_F32)
-                    load4<float>(static_cast<const float*>(p.q) + off, p.vec, x[i]);
-                else if (p.type == T_F16)
-                    load4<__half>(static_cast<const __half*>(p.q) + off, p.vec, x[i]);
-                else
-                    load4<__nv_bfloat16>(static_cast<const __nv_bfloat16*>(p.q) + off, p.vec, x[i]);
+                load4<T>(static_cast<const T*>(p.q) + off, p.vec, x[i]);
             }
         };
         float qx[kRows][4];
@@ -607,13 +681,12 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
                         if constexpr (C == 8) tmem_ld8(tm + sb * N + d * RT + r0, c[d]);
                         else tmem_ld4(tm + sb * N + d * RT + r0, c[d]);
                     }
+                    float qs[C];
+                    load_rows<C>(&z.qscale[sg][r0], qs);
                     tmem_wait();
 #pragma unroll
                     for (int r = 0; r < C; ++r) {
-                        float v = (float)c[0][r];
-#pragma unroll
-                        for (int d = 1; d < DG; ++d) v = fmaf(v, 256.0f, (float)c[d][r]);
-                        x[r0 + r] = v * (z.qscale[sg][r0 + r] * ks);
+                        x[r0 + r] = digits_value<DG, C>(c, r) * (qs[r] * ks);
                     }
                 }
                 fence_before();
@@ -633,8 +706,8 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
                 float mx[RT];
 #pragma unroll
                 for (int r = 0; r < RT; ++r) mx[r] = warp_max_nan(x[r]);
-                if (P > 32) {  // the page spans several warps
-                    const int w0 = P == 64 ? warp & 2 : 0, wn = P / 32;
+                if (lgP > 5) {  // the page spans several warps
+                    const int w0 = lgP == 6 ? warp & 2 : 0, wn = 1 << (lgP - 5);
                     if (lane == 0) {
                         store_rows<RT>(z.wmax[pb][warp], mx);
                         mbar_arrive(&br.pmax[pb][w0 >> 1]);
@@ -674,8 +747,7 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
                         pt[(n0)*128 + sw * 16] = (uint8_t)(d >> 8);
                         pt[(n0 + RT) * 128 + ((tid >> 4) ^ ((n0 + RT) & 7)) * 16] = (uint8_t)d;
                     }
-                    // u - 0x3f800000 per lane
-                    sum[r] = (float)(__reduce_add_sync(~0u, u) - 32u * 0x3f800000u) * (1.0f / 8388608.0f);
+                    sum[r] = __uint_as_float(__reduce_add_sync(~0u, u));
                 }
                 if (lane == 0) {
                     store_rows<RT>(z.stat_sum[pb][warp], sum);
@@ -702,6 +774,7 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
         constexpr float kUnit = DG == 3 ? 1.0f / 8388608.0f : 1.0f / 65536.0f;
         constexpr size_t kPart = RT * 130;
         const int me = blockIdx.x;
+        T* out = static_cast<T*>(p.out);
         // Offsets of the row tile's rows, in lane r that of row r (-1: no such
         // row); element `e` of a row from there.
         auto row_of = [&](const Seg& k, long long& off, long long& lse) {
@@ -710,24 +783,21 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
             off = qi < k.n ? row * p.ldo + (long long)hq * p.w.hd : -1;
             lse = row * p.H + hq;
         };
-        auto put = [&](long long off, float v) {
-            if (p.type == QUANTR_TYPE_F32) static_cast<float*>(p.out)[off] = v;
-            else if (p.type == T_F16) static_cast<__half*>(p.out)[off] = __float2half_rn(v);
-            else static_cast<__nv_bfloat16*>(p.out)[off] = __float2bfloat16_rn(v);
-        };
         auto lse_of = [&](float m, float l) {
             return m == -INFINITY ? m : (m + log2f(l) + (DG == 3 ? 0.0f : 2.2013990e-5f)) * 0.693147180559945f;
         };
         // Counts this CTA in; true in all join threads if it is the last of n,
         // and then the others' parts can be read.
         auto last_of = [&](int* counter, int n, bool& last) -> bool {
-            __threadfence();
+            // The barrier orders the join threads' parts before the counting
+            // (release, cumulative), the counting the others' before the reads.
             __syncwarp();
             if (lane == 0) mbar_arrive(&br.jdone);
             if (tid == 0 && mbar_wait_bounded(&br.jdone, meets & 1, err, abort)) {
-                z.last = atomicAdd(counter, 1) == n - 1;
+                int old;
+                asm volatile("atom.add.acq_rel.gpu.s32 %0, [%1], 1;" : "=r"(old) : "l"(counter) : "memory");
+                z.last = old == n - 1;
                 if (z.last) *counter = 0;
-                __threadfence();
                 mbar_arrive(&br.jlast);
             }
             __syncwarp();
@@ -749,7 +819,7 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
                 if (!(ok = warp_wait(&br.stfull[sb], su & 1, err, abort))) break;
                 if (lane < RT) {
                     float mp[4], mn = m_run;
-                    const int per = P / 32;
+                    const int per = 1 << (lgP - 5);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         mp[j] = j < NP ? z.stat_max[sb][j * per][lane] : -INFINITY;
@@ -764,8 +834,8 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
                         if (j < NP) {
                             const float f = ex2(mp[j] - ref);
                             float sum = 0.0f;
-                            for (int w = j * per; w < (j + 1) * per; ++w) sum += z.stat_sum[sb][w][lane];
-                            l_run = fmaf(sum, f, l_run);
+                            for (int w = j * per; w < (j + 1) * per; ++w) sum += (float)(__float_as_uint(z.stat_sum[sb][w][lane]) - 32u * 0x3f800000u);
+                            l_run = fmaf(sum * (1.0f / 8388608.0f), f, l_run);
                             // A page that is masked altogether counts nothing, whatever its scale.
                             z.join[w4][1 + j][lane] = mp[j] == -INFINITY ? 0.0f : f * kUnit * z.stat_vs[sb][j];
                         }
@@ -775,8 +845,12 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
                 if (lane == 0) mbar_arrive(&br.stempty[sb]);
                 if (!(ok = warp_wait(&br.ofull[ob], ou & 1, err, abort))) break;
                 fence_after();
+                {
+                    float w[RT];
+                    load_rows<RT>(z.join[w4][0], w);
 #pragma unroll
-                for (int r = 0; r < RT; ++r) o[r] *= z.join[w4][0][r];
+                    for (int r = 0; r < RT; ++r) o[r] *= w[r];
+                }
                 for (int j = 0; j < NP; ++j) {
 #pragma unroll
                     for (int r0 = 0; r0 < RT; r0 += (RT < 8 ? RT : 8)) {
@@ -787,13 +861,12 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
                             if constexpr (C == 8) tmem_ld8(tm + (ob * NP + j) * N + d * RT + r0, c[d]);
                             else tmem_ld4(tm + (ob * NP + j) * N + d * RT + r0, c[d]);
                         }
+                        float w[C];
+                        load_rows<C>(&z.join[w4][1 + j][r0], w);
                         tmem_wait();
 #pragma unroll
                         for (int r = 0; r < C; ++r) {
-                            float v = (float)c[0][r];
-#pragma unroll
-                            for (int d = 1; d < DG; ++d) v = fmaf(v, 256.0f, (float)c[d][r]);
-                            o[r0 + r] = fmaf(v, z.join[w4][1 + j][r0 + r], o[r0 + r]);
+                            o[r0 + r] = fmaf(digits_value<DG, C>(c, r), w[r], o[r0 + r]);
                         }
                     }
                 }
@@ -813,7 +886,7 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
                 for (int r = 0; r < RT; ++r) {
                     const long long to = __shfl_sync(~0u, off, r);
                     const float v = o[r] * __shfl_sync(~0u, inv, r);
-                    if (to >= 0 && tid < p.w.hd) put(to + tid, v);
+                    if (to >= 0 && tid < p.w.hd) out[to + tid] = from_f<T>(v);
                 }
             } else {
                 // A part: o[RT][128], m[RT], l[RT].
@@ -826,43 +899,52 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
             }
         }
         // Joins the n <= 32 parts at base, base + stride, ... (the first of them
-        // one part further when `shift`), row by row: warp w4 takes the rows w4,
-        // w4 + 4, ...; lane i weighs part i, and has 4 of the row's elements.
+        // one part further when `shift`), 8 rows at a time: 16 threads have a
+        // row, 8 elements each, and lanes j of them weigh the parts j and 16 + j.
         // To another part, or (null) to the output.
         auto join_parts = [&](const float* base, int n, size_t stride, bool shift, float* to, const Seg& k) {
             long long off, at;
             row_of(k, off, at);
+            const int j = tid & 15, head = lane & 16;
 #pragma unroll 1
-            for (int r = w4; r < RT; r += 4) {
-                const float* mine = base + lane * stride + (shift && lane == 0 ? kPart : 0) + RT * 128 + r;
-                float m = -INFINITY, l = 0.0f;
-                if (lane < n) m = __ldcg(mine), l = __ldcg(mine + RT);
-                const float top = warp_max_nan(m), f = ex2(m - (top == -INFINITY ? 0.0f : top));
-                l *= f;
+            for (int r0 = 0; r0 < RT; r0 += 8) {
+                const int r = min(r0 + (tid >> 4), RT - 1);
+                const float* row = base + (shift ? kPart : 0);  // of part 0; the others lie one part lower
+                auto part_at = [&](int i) { return i ? base + i * stride : row; };
+                float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+                const float* mine = part_at(j) + RT * 128 + r;
+                if (j < n) m0 = __ldcg(mine), l0 = __ldcg(mine + RT);
+                if (16 + j < n) m1 = __ldcg(base + (16 + j) * stride + RT * 128 + r), l1 = __ldcg(base + (16 + j) * stride + RT * 129 + r);
+                float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f), b = a;
+                float top = max_nan(m0, m1);
 #pragma unroll
-                for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(~0u, l, d);
-                float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                for (int d = 8; d; d >>= 1) top = max_nan(top, __shfl_xor_sync(~0u, top, d));
+                const float ref = top == -INFINITY ? 0.0f : top, f0 = ex2(m0 - ref), f1 = ex2(m1 - ref);
+                float l = fmaf(l0, f0, l1 * f1);
+#pragma unroll
+                for (int d = 8; d; d >>= 1) l += __shfl_xor_sync(~0u, l, d);
 #pragma unroll 4
                 for (int i = 0; i < n; ++i) {
-                    const float4 v = __ldcg(reinterpret_cast<const float4*>(
-                        base + i * stride + (shift && i == 0 ? kPart : 0) + r * 128 + lane * 4));
-                    const float g = __shfl_sync(~0u, f, i);
-                    o.x = fmaf(v.x, g, o.x), o.y = fmaf(v.y, g, o.y), o.z = fmaf(v.z, g, o.z), o.w = fmaf(v.w, g, o.w);
+                    const float4* v = reinterpret_cast<const float4*>(part_at(i) + r * 128 + j * 8);
+                    const float4 x = __ldcg(v), y = __ldcg(v + 1);
+                    const float g = __shfl_sync(~0u, i < 16 ? f0 : f1, head | (i & 15));
+                    a.x = fmaf(x.x, g, a.x), a.y = fmaf(x.y, g, a.y), a.z = fmaf(x.z, g, a.z), a.w = fmaf(x.w, g, a.w);
+                    b.x = fmaf(y.x, g, b.x), b.y = fmaf(y.y, g, b.y), b.z = fmaf(y.z, g, b.z), b.w = fmaf(y.w, g, b.w);
                 }
+                const long long o_at = __shfl_sync(~0u, off, r), l_at = __shfl_sync(~0u, at, r);
+                if (r0 + (tid >> 4) >= RT) continue;
                 if (to) {
-                    *reinterpret_cast<float4*>(to + r * 128 + lane * 4) = o;
-                    if (lane == 0) to[RT * 128 + r] = top, to[RT * 129 + r] = l;
-                    continue;
-                }
-                const long long row = __shfl_sync(~0u, off, r), lse = __shfl_sync(~0u, at, r);
-                if (row < 0) continue;
-                const float inv = 1.0f / l;
-                const float v[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
-                if (lane * 4 < p.w.hd) {
+                    float4* t = reinterpret_cast<float4*>(to + r * 128 + j * 8);
+                    t[0] = a, t[1] = b;
+                    if (j == 0) to[RT * 128 + r] = top, to[RT * 129 + r] = l;
+                } else if (o_at >= 0) {
+                    const float inv = top == -INFINITY ? 0.0f : 1.0f / l;
+                    const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) put(row + lane * 4 + j, top == -INFINITY ? 0.0f : v[j]);
+                    for (int e = 0; e < 8; ++e)
+                        if (j * 8 + e < p.w.hd) out[o_at + j * 8 + e] = from_f<T>(v[e] * inv);
+                    if (p.lse && j == 0) p.lse[l_at] = lse_of(top, l);
                 }
-                if (p.lse && lane == 0) p.lse[lse] = lse_of(top, l);
             }
         };
         // Shared row tiles: whoever comes last joins them, in token order.
@@ -970,29 +1052,29 @@ bool encode_map(CUtensorMap* map, const void* base, const quantr_kv8_pool* p, in
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int DG, int RT, int HDW>
+template <typename T, int RT, int HDW>
 cudaError_t run(AttendParams& p, const quantr_kv8_pool* pool, void* ws, const LaunchCfg& c)
 {
-    const Plan r = make_plan<DG, RT, HDW>(p.w.lgP);
+    const Plan r = make_plan<digits<T>, RT, HDW>(p.w.lgP);
     static int configured = -1;
-    cudaError_t e = ensure_smem_attr(k_kv8_attend<DG, RT, HDW>, 227 * 1024, configured);
+    cudaError_t e = ensure_smem_attr(k_kv8_attend<T, RT, HDW>, 227 * 1024, configured);
     if (e != cudaSuccess) return e;
     if (!encode_map(&p.kmap, pool->k, pool, HDW) || !encode_map(&p.vmap, pool->v, pool, HDW))
         return cudaErrorNotSupported;
-    p.stages = r.stages, p.nS = r.nS, p.nO = r.nO, p.tmem_cols = r.cols, p.min_share = 2;
+    p.stages = r.stages, p.nS = r.nS, p.nO = r.nO, p.tmem_cols = r.cols;
     p.counters = static_cast<int*>(ws);
     p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + 4096);
-    return launch_ex(k_kv8_attend<DG, RT, HDW>, dim3(r.grid), kThreads, r.smem, c, p);
+    return launch_ex(k_kv8_attend<T, RT, HDW>, dim3(r.grid), kThreads, r.smem, c, p);
 }
 
-template <int DG, int HDW>
+template <typename T, int HDW>
 cudaError_t run_rt(int rt, AttendParams& p, const quantr_kv8_pool* pool, void* ws, const LaunchCfg& c)
 {
     switch (rt) {
-    case 4: return run<DG, 4, HDW>(p, pool, ws, c);
-    case 8: return run<DG, 8, HDW>(p, pool, ws, c);
-    case 16: return run<DG, 16, HDW>(p, pool, ws, c);
-    default: return run<DG, 32, HDW>(p, pool, ws, c);
+    case 4: return run<T, 4, HDW>(p, pool, ws, c);
+    case 8: return run<T, 8, HDW>(p, pool, ws, c);
+    case 16: return run<T, 16, HDW>(p, pool, ws, c);
+    default: return run<T, 32, HDW>(p, pool, ws, c);
     }
 }
 
@@ -1036,18 +1118,17 @@ int quantr_kv8_attend_dev(void* out, long long ldo, const void* q, long long ldq
     }
     AttendParams p{};
     p.w = kv8_view(pool, tables, batch, layer);
-    p.q = q, p.out = out, p.lse = lse, p.ldq = ldq, p.ldo = ldo, p.type = type;
+    p.q = q, p.out = out, p.lse = lse, p.ldq = ldq, p.ldo = ldo;
     p.vec = aligned4(q, ldq, type == QUANTR_TYPE_F32 ? 4 : 2);
     p.H = n_heads, p.G = n_heads / pool->n_kv_heads, p.window = window;
     p.inv_g = p.G == 1 ? 0 : (unsigned)(((1ull << 32) + p.G - 1) / p.G);
     p.scale2 = (float)((double)scale * 1.4426950408889634);
     LaunchCfg c;
     c.stream = (cudaStream_t)stream;
-    cudaError_t e;
-    if (type == QUANTR_TYPE_F32)
-        e = pool->head_dim <= 64 ? run_rt<3, 64>(rt, p, pool, workspace, c) : run_rt<3, 128>(rt, p, pool, workspace, c);
-    else
-        e = pool->head_dim <= 64 ? run_rt<2, 64>(rt, p, pool, workspace, c) : run_rt<2, 128>(rt, p, pool, workspace, c);
+    const cudaError_t e = with_type(type, [&](auto* t) {
+        using T = std::remove_const_t<std::remove_pointer_t<decltype(t)>>;
+        return pool->head_dim <= 64 ? run_rt<T, 64>(rt, p, pool, workspace, c) : run_rt<T, 128>(rt, p, pool, workspace, c);
+    });
     return kv8_done(e);
 }
 
