@@ -322,7 +322,7 @@ struct Shape {
 
 struct Bars {
     uint64_t kfull[kMaxStages], kempty[kMaxStages], vfull[kMaxStages], vempty[kMaxStages];
-    uint64_t sfull[2], sempty[2], pfull[2], pempty[2], ofull[2], oempty[2], stfull[2], stempty[2];
+    uint64_t sfull[2], sempty[2], pfull[2], ofull[2], joined[2];
     uint64_t mfull[kMeta], segfull[kMeta], qfull, pmax[2][2], jdone, jlast;
 };
 
@@ -340,7 +340,7 @@ struct alignas(16) Small {
     float qscale[2][RT];  // by the segment's parity
     int pos[2][RT];
     float join[4][5][RT];      // per join warp: the factor of what was there, then of each page
-    float stat_vs[2][4];
+    float stat_vs[2][4];  // and its page's scale of v
     Meta meta[kMeta];
     Seg seg[kMeta];
     Bars bars;
@@ -414,11 +414,8 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
             mbar_init(&br.sfull[i], 1);
             mbar_init(&br.sempty[i], 4);
             mbar_init(&br.pfull[i], 4);
-            mbar_init(&br.pempty[i], 1);
             mbar_init(&br.ofull[i], 1);
-            mbar_init(&br.oempty[i], 4);
-            mbar_init(&br.stfull[i], 4);
-            mbar_init(&br.stempty[i], 4);
+            mbar_init(&br.joined[i], 4);
         }
         for (int i = 0; i < kMeta; ++i) {
             mbar_init(&br.mfull[i], 1);
@@ -532,7 +529,7 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
         // ------------------------------------------------------------ MMAs --
         const uint32_t idS = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | (8u << 24);
         const uint32_t idO = (2u << 4) | (1u << 7) | (1u << 15) | ((uint32_t)(N >> 3) << 17) | (8u << 24);
-        int kst = 0, kuse = 0, vst = 0, vuse = 0, sb = 0, su = 0, pb = 0, pu = 0, ob = 0, ou = 0, seg = 0;
+        int kst = 0, kuse = 0, vst = 0, vuse = 0, sb = 0, su = 0, pb = 0, pu = 0, ob = 0, ou = 0, seg = 0, tile = 0;
         // An address moves a descriptor by its sixteenth.
         const uint64_t qd = desc_of(sptr(qsm), 8 * HDW, kSw), kd = desc_of(sptr(ksm), 8 * HDW, kSw);
         const uint64_t vd = desc_of(sptr(vsm), 8 * HDW, kSw), pd = desc_of(sptr(psm), 1024, 2u);
@@ -558,7 +555,11 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
         auto issue_o = [&]() -> bool {
             if (!warp_wait(&br.vfull[vst], vuse & 1, err, abort) || !warp_wait(&br.pfull[pb], pu & 1, err, abort))
                 return false;
-            if (ou > 0 && !warp_wait(&br.oempty[ob], (ou - 1) & 1, err, abort)) return false;
+            // The outputs' buffer: of the tile before the last, or of the last.
+            if (p.nO == 2 ? pu > 0 : tile > 0) {
+                const int of = p.nO == 2 ? tile - 2 : tile - 1;
+                if (!warp_wait(&br.joined[of & 1], of >> 1 & 1, err, abort)) return false;
+            }
             fence_after();
             if (elect()) {
 #pragma unroll
@@ -566,7 +567,6 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
                     mma_i8(tm_o + (ob * NP + (i >> lg_per)) * N, vd + (uint32_t)(vst * (kStage / 16) + 2 * HDW * i),
                            pd + (uint32_t)(pb * (kPBytes / 16) + 2 * i), idO, (i & first_of) > 0);
                 mma_commit(&br.ofull[ob]);
-                mma_commit(&br.pempty[pb]);
                 mma_commit(&br.vempty[vst]);
             }
             __syncwarp();
@@ -574,6 +574,7 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
             if (++vst == S) vst = 0, ++vuse;
             if (++pb == 2) pb = 0, ++pu;
             if (++ob == p.nO) ob = 0, ++ou;
+            ++tile;
             return true;
         };
         Seg k;
@@ -581,8 +582,12 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
         while (ok && more) {
             const int t1 = k.t1;
             for (int t = k.t0; ok && t < t1; ++t) {
-                if (t + 1 < t1) ok = issue_s(false);
+                // The next scores first, unless their keys are still on the way:
+                // then this tile's outputs, which free its values' stage.
+                const bool first = t + 1 < t1 && __all_sync(~0u, mbar_try_wait(&br.kfull[kst], kuse & 1));
+                if (first) ok = issue_s(false);
                 ok = ok && issue_o();
+                if (!first && t + 1 < t1) ok = ok && issue_s(false);
             }
             if (!ok || !(more = next_seg(k))) break;
             ok = issue_s(true);
@@ -621,9 +626,9 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
                 const float top = warp_max_nan(max_nan(max_nan(fabsf(x[0]), fabsf(x[1])), max_nan(fabsf(x[2]), fabsf(x[3]))));
                 const bool fine = top <= 3.402823466e38f;
                 // The largest power of two that keeps the row's largest element
-                // in range.  Below 1e-30 every score rounds to 0 anyway.
+                // in range.  Below 3e-32 (no power of two for it) rows count as 0.
                 float inv = 0.0f, step = 0.0f;
-                if (fine && top > 1e-30f) {
+                if (fine && top > 3e-32f) {
                     const int ex = 252 + 8 * DG - (int)(__float_as_uint(top) >> 23);
                     inv = __uint_as_float((uint32_t)ex << 23);
                     if (top * inv > kQMax) inv *= 0.5f;
@@ -660,6 +665,7 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
             const int pos_lo = z.pos[sg][0], pos_hi = z.pos[sg][RT - 1];
 
             const int t0 = k.t0, t1 = k.t1;
+#pragma unroll 1
             for (int t = t0; t < t1; ++t) {
                 if (t + 1 == t1) {  // the next row tile's rows come during the last tile
                     more = next_seg(k);
@@ -671,7 +677,7 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
                 const float ks = m.ks[page];
                 const int valid = m.valid;
                 fence_after();
-                float x[RT];
+                float x[RT], mx[RT];
 #pragma unroll
                 for (int r0 = 0; r0 < RT; r0 += (RT < 8 ? RT : 8)) {
                     constexpr int C = RT < 8 ? RT : 8;
@@ -685,9 +691,7 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
                     load_rows<C>(&z.qscale[sg][r0], qs);
                     tmem_wait();
 #pragma unroll
-                    for (int r = 0; r < C; ++r) {
-                        x[r0 + r] = digits_value<DG, C>(c, r) * (qs[r] * ks);
-                    }
+                    for (int r = 0; r < C; ++r) x[r0 + r] = digits_value<DG, C>(c, r) * (qs[r] * ks);
                 }
                 fence_before();
                 __syncwarp();
@@ -703,7 +707,6 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
                         x[r] = seen ? x[r] : -INFINITY;
                     }
                 }
-                float mx[RT];
 #pragma unroll
                 for (int r = 0; r < RT; ++r) mx[r] = warp_max_nan(x[r]);
                 if (lgP > 5) {  // the page spans several warps
@@ -713,6 +716,7 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
                         mbar_arrive(&br.pmax[pb][w0 >> 1]);
                     }
                     if (!(ok = warp_wait(&br.pmax[pb][w0 >> 1], pu & 1, err, abort))) break;
+#pragma unroll 1
                     for (int w = w0; w < w0 + wn; ++w) {
 #pragma unroll
                         for (int r = 0; r < RT; r += 4) {
@@ -722,11 +726,9 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
                         }
                     }
                 }
-                if (pu > 0) {
-                    ok = warp_wait(&br.pempty[pb], (pu - 1) & 1, err, abort) &&
-                         warp_wait(&br.stempty[pb], (pu - 1) & 1, err, abort);
-                    if (!ok) break;
-                }
+                // The tile before the last is joined: its weights were used and
+                // its maxima read.
+                if (pu > 0 && !(ok = warp_wait(&br.joined[pb], (pu - 1) & 1, err, abort))) break;
                 float sum[RT];
                 uint8_t* pt = psm + pb * kPBytes + (tid & 15);
 #pragma unroll
@@ -738,28 +740,26 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
                     const float w = ex2(DG == 3 ? x[r] - ref : x[r] - ref - 2.2013990e-5f);
                     const uint32_t u = __float_as_uint(1.0f + w);
                     const uint32_t d = DG == 3 ? u : __float_as_uint(128.0f + w);
-                    const int n0 = r, sw = (tid >> 4) ^ (r & 7);
+                    auto put = [&](int n, uint32_t v) { pt[n * 128 + (((tid >> 4) ^ (n & 7)) << 4)] = (uint8_t)v; };
                     if constexpr (DG == 3) {
-                        pt[(n0)*128 + sw * 16] = (uint8_t)((d >> 16) - 0x80);
-                        pt[(n0 + RT) * 128 + ((tid >> 4) ^ ((n0 + RT) & 7)) * 16] = (uint8_t)(d >> 8);
-                        pt[(n0 + 2 * RT) * 128 + ((tid >> 4) ^ ((n0 + 2 * RT) & 7)) * 16] = (uint8_t)d;
+                        put(r, (d >> 16) - 0x80);
+                        put(r + RT, d >> 8);
+                        put(r + 2 * RT, d);
                     } else {
-                        pt[(n0)*128 + sw * 16] = (uint8_t)(d >> 8);
-                        pt[(n0 + RT) * 128 + ((tid >> 4) ^ ((n0 + RT) & 7)) * 16] = (uint8_t)d;
+                        put(r, d >> 8);
+                        put(r + RT, d);
                     }
+                    // u - 0x3f800000 per lane
                     sum[r] = __uint_as_float(__reduce_add_sync(~0u, u));
                 }
                 if (lane == 0) {
                     store_rows<RT>(z.stat_sum[pb][warp], sum);
                     store_rows<RT>(z.stat_max[pb][warp], mx);
+                    z.stat_vs[pb][warp] = m.vs[page];
                 }
-                if (tid < NP) z.stat_vs[pb][tid] = m.vs[tid];
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(&br.pfull[pb]);
-                    mbar_arrive(&br.stfull[pb]);
-                }
+                if (lane == 0) mbar_arrive(&br.pfull[pb]);
                 if (++sb == p.nS) sb = 0, ++su;
                 if (++pb == 2) pb = 0, ++pu;
                 if (++mt == kMeta) mt = 0, ++mu;
@@ -770,9 +770,10 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
         const int tid = threadIdx.x - 128, w4 = warp - 4;
         const uint32_t tm = tm_o + ((uint32_t)w4 << 21);
         int sb = 0, su = 0, ob = 0, ou = 0, meets = 0;
-        bool ok = true, more = true;
+        bool ok = true;
         constexpr float kUnit = DG == 3 ? 1.0f / 8388608.0f : 1.0f / 65536.0f;
         constexpr size_t kPart = RT * 130;
+        constexpr int kSets = RT <= 8 ? 1 : RT / 8, kSet = RT < 8 ? RT : 8;
         const int me = blockIdx.x;
         T* out = static_cast<T*>(p.out);
         // Offsets of the row tile's rows, in lane r that of row r (-1: no such
@@ -814,35 +815,36 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
             float o[RT];
 #pragma unroll
             for (int r = 0; r < RT; ++r) o[r] = 0.0f;
-            float m_run = -INFINITY, l_run = 0.0f;  // lane r: of row r
+            // Lane 8 w + r has softmax warp w's part of rows r, 8 + r, ...
+            float m_run[kSets], l_run[kSets];
+#pragma unroll
+            for (int i = 0; i < kSets; ++i) m_run[i] = -INFINITY, l_run[i] = 0.0f;
             for (int t = k.t0; t < k.t1; ++t) {
-                if (!(ok = warp_wait(&br.stfull[sb], su & 1, err, abort))) break;
-                if (lane < RT) {
-                    float mp[4], mn = m_run;
-                    const int per = 1 << (lgP - 5);
+                if (!(ok = warp_wait(&br.pfull[sb], su & 1, err, abort))) break;
+                const int from = lane >> 3;
+                const float vs = z.stat_vs[sb][from];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        mp[j] = j < NP ? z.stat_max[sb][j * per][lane] : -INFINITY;
-                        mn = max_nan(mn, mp[j]);
+                for (int i = 0; i < kSets; ++i) {
+                    const int r = 8 * i + (lane & (kSet - 1));
+                    const float mp = z.stat_max[sb][from][r];
+                    const float sum = (float)(__float_as_uint(z.stat_sum[sb][from][r]) - 32u * 0x3f800000u);
+                    float mn = max_nan(m_run[i], mp);
+                    mn = max_nan(mn, __shfl_xor_sync(~0u, mn, 8));
+                    mn = max_nan(mn, __shfl_xor_sync(~0u, mn, 16));
+                    const float ref = mn == -INFINITY ? 0.0f : mn, f = ex2(mp - ref), a = ex2(m_run[i] - ref);
+                    float l = sum * (1.0f / 8388608.0f) * f;
+                    l += __shfl_xor_sync(~0u, l, 8);
+                    l += __shfl_xor_sync(~0u, l, 16);
+                    l_run[i] = fmaf(l_run[i], a, l);
+                    m_run[i] = mn;
+                    if ((lane & 7) < kSet) {
+                        if (lane < 8) z.join[w4][0][r] = a;
+                        // A page that is masked altogether counts nothing, whatever its scale.
+                        if ((from & ((1 << (lgP - 5)) - 1)) == 0)
+                            z.join[w4][1 + (from >> (lgP - 5))][r] = mp == -INFINITY ? 0.0f : f * kUnit * vs;
                     }
-                    const float ref = mn == -INFINITY ? 0.0f : mn;
-                    const float a = ex2(m_run - ref);
-                    l_run *= a;
-                    z.join[w4][0][lane] = a;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (j < NP) {
-                            const float f = ex2(mp[j] - ref);
-                            float sum = 0.0f;
-                            for (int w = j * per; w < (j + 1) * per; ++w) sum += (float)(__float_as_uint(z.stat_sum[sb][w][lane]) - 32u * 0x3f800000u);
-                            l_run = fmaf(sum * (1.0f / 8388608.0f), f, l_run);
-                            // A page that is masked altogether counts nothing, whatever its scale.
-                            z.join[w4][1 + j][lane] = mp[j] == -INFINITY ? 0.0f : f * kUnit * z.stat_vs[sb][j];
-                        }
-                    m_run = mn;
                 }
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&br.stempty[sb]);
                 if (!(ok = warp_wait(&br.ofull[ob], ou & 1, err, abort))) break;
                 fence_after();
                 {
@@ -872,16 +874,23 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
                 }
                 fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&br.oempty[ob]);
+                if (lane == 0) mbar_arrive(&br.joined[sb]);
                 if (++sb == 2) sb = 0, ++su;
                 if (++ob == p.nO) ob = 0, ++ou;
             }
             if (!ok) break;
+            // Lane r: row r.
+            float m_row = m_run[0], l_row = l_run[0];
+#pragma unroll
+            for (int i = 1; i < kSets; ++i) {
+                const float m = __shfl_sync(~0u, m_run[i], lane & 7), l = __shfl_sync(~0u, l_run[i], lane & 7);
+                if (lane >> 3 == i) m_row = m, l_row = l;
+            }
             if (k.c0 == k.c1) {
                 long long off, at;
                 row_of(k, off, at);
-                const float inv = m_run == -INFINITY ? 0.0f : 1.0f / l_run;  // nothing seen: o is 0
-                if (p.lse && w4 == 0 && lane < RT && off >= 0) p.lse[at] = lse_of(m_run, l_run);
+                const float inv = m_row == -INFINITY ? 0.0f : 1.0f / l_row;  // nothing seen: o is 0
+                if (p.lse && w4 == 0 && lane < RT && off >= 0) p.lse[at] = lse_of(m_row, l_row);
 #pragma unroll
                 for (int r = 0; r < RT; ++r) {
                     const long long to = __shfl_sync(~0u, off, r);
@@ -893,7 +902,7 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
                 float* part = p.part + (2 * (size_t)me + (me == k.c0 ? 1 : 0)) * kPart;
 #pragma unroll
                 for (int r = 0; r < RT; ++r) part[r * 128 + tid] = o[r];
-                if (w4 == 0 && lane < RT) part[RT * 128 + lane] = m_run, part[RT * 129 + lane] = l_run;
+                if (w4 == 0 && lane < RT) part[RT * 128 + lane] = m_row, part[RT * 129 + lane] = l_row;
                 if (n_shared++) shared1 = k;
                 else shared0 = k;
             }
