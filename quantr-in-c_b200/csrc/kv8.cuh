@@ -219,6 +219,10 @@ inline bool aligned4(const void* p, long long ld, int bytes)
     return ((uintptr_t)p % (4 * bytes)) == 0 && ld % 4 == 0;
 }
 
+// Whether head slices of such rows (whole multiples of 16 elements) allow
+// 16-byte loads.
+inline bool aligned16(const void* p, long long ld, int bytes) { return ((uintptr_t)p & 15) == 0 && ld * bytes % 16 == 0; }
+
 // Calls f with a null T* of the element type.
 template <typename F>
 cudaError_t with_type(uint32_t type, F&& f)

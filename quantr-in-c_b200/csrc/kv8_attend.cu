@@ -211,7 +211,7 @@ __device__ __forceinline__ void walk_enter(const AttendParams& p, Walk& k)
 // This CTA's part of the work and its first segment.  Two ways to share it out:
 //   by row tiles, where there are no more of them than CTAs and their lengths
 //   differ little: a row tile has `per` CTAs, each with one run of its tiles
-//   (at least sqrt(nt/6): a part costs the join about a sixth of a tile);
+//   (at least sqrt(nt/12): a part costs the join about a twelfth of a tile);
 //   by tiles, else: equal runs of the flat list of all tiles.
 // Lane l looks at the sequences 32 i + l.
 template <int RT>
@@ -287,7 +287,7 @@ __device__ __forceinline__ void walk_begin(const AttendParams& p, Walk& k)
         k.s = kv8_seq(p.w, k.b);
         seq_tiles<RT>(p, k.s, k.nrt, k.nt, k.tlo);
         const int item = k.pos - k.first;
-        const int run = max((k.nt + per - 1) / per, (int)ceilf(sqrtf((float)k.nt * (1.0f / 6.0f))));
+        const int run = max((k.nt + per - 1) / per, (int)ceilf(sqrtf((float)k.nt * (1.0f / 12.0f))));
         k.seg.h = item / k.nrt;
         k.seg.rt = item - k.seg.h * k.nrt;
         k.seg.row0 = k.s.row0, k.seg.n = k.s.n, k.seg.len = k.s.len;

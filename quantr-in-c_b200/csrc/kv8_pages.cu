@@ -47,37 +47,42 @@ struct SelectArgs {
     int* err;
 };
 
-__global__ void __launch_bounds__(256) k_kv8_zero(int* p, int n)
-{
-    pdl_wait();
-    for (int i = blockIdx.x * 256 + threadIdx.x; i < n; i += gridDim.x * 256) p[i] = 0;
-}
+constexpr int kSelectCtas = 8, kSelectThreads = 1024;
 
-// One CTA per slot.
-__global__ void __launch_bounds__(128) k_kv8_select(const SelectArgs a)
+// One cluster: the references are zeroed, the cluster meets, and its warps take
+// the slots one by one, counting the pages they copy.  One launch: 4 us for 64
+// slots of 20 pages.  (Integer counts: their order does not matter.)
+__global__ void __launch_bounds__(kSelectThreads) __cluster_dims__(kSelectCtas, 1, 1) k_kv8_select(const SelectArgs a)
 {
     pdl_wait();
-    const int s = blockIdx.x, P = 1 << a.lgP;
-    int f = a.from[s];
-    if (f < -1 || f >= a.in.slots) {
-        kv8_fault(a.err);
-        f = -1;
-    }
-    int len = f >= 0 ? a.in.lens[f] : 0;
-    if (len < 0 || (long long)len > ((long long)a.in.max_pages << a.lgP)) {
-        kv8_fault(a.err);
-        len = 0;
-    }
-    const int used = (int)(((long long)len + P - 1) >> a.lgP);
-    for (int i = threadIdx.x; i < a.in.max_pages; i += 128) {
-        const int page = i < used ? a.in.table[(size_t)f * a.in.max_pages + i] : -1;
-        a.to.table[(size_t)s * a.to.max_pages + i] = page;
-        if (page >= 0 && page < a.n_pages)
-            atomicAdd(a.to.refs + page, 1);
-        else if (i < used)
+    const int lane = threadIdx.x & 31, P = 1 << a.lgP;
+    for (int i = blockIdx.x * kSelectThreads + threadIdx.x; i < a.n_pages; i += kSelectCtas * kSelectThreads)
+        a.to.refs[i] = 0;
+    cluster_arrive();
+    cluster_wait();
+    for (int s = (blockIdx.x * kSelectThreads + threadIdx.x) >> 5; s < a.to.slots; s += kSelectCtas * kSelectThreads / 32) {
+        int f = a.from[s];
+        if (f < -1 || f >= a.in.slots) {
             kv8_fault(a.err);
+            f = -1;
+        }
+        int len = f >= 0 ? a.in.lens[f] : 0;
+        if (len < 0 || (long long)len > ((long long)a.in.max_pages << a.lgP)) {
+            kv8_fault(a.err);
+            len = 0;
+        }
+        const int used = (int)(((long long)len + P - 1) >> a.lgP);
+        const int* in = a.in.table + (size_t)max(f, 0) * a.in.max_pages;
+        int* to = a.to.table + (size_t)s * a.to.max_pages;
+#pragma unroll 4
+        for (int i = lane; i < a.in.max_pages; i += 32) {
+            const int page = i < used ? in[i] : -1;
+            to[i] = page;
+            if (page >= 0 && page < a.n_pages) atomicAdd(a.to.refs + page, 1);
+            else if (i < used) kv8_fault(a.err);
+        }
+        if (lane == 0) a.to.lens[s] = len;
     }
-    if (threadIdx.x == 0) a.to.lens[s] = len;
 }
 
 // ----------------------------------------------------------- page copying --
@@ -97,39 +102,44 @@ struct CopyArgs {
     size_t entries;
 };
 
-__device__ __forceinline__ void copy_span(void* d, const void* s, size_t bytes, size_t at, size_t step)
-{
-    if ((((uintptr_t)d | (uintptr_t)s | bytes) & 15) == 0) {
-        uint4* dd = static_cast<uint4*>(d);
-        const uint4* ss = static_cast<const uint4*>(s);
-        for (size_t i = at; i < bytes / 16; i += step) dd[i] = ss[i];
-    } else {
-        uint32_t* dd = static_cast<uint32_t*>(d);
-        const uint32_t* ss = static_cast<const uint32_t*>(s);
-        for (size_t i = at; i < bytes / 4; i += step) dd[i] = ss[i];
-    }
-}
+constexpr int kAtOnce = 8;                                  // 16-byte loads in flight per thread
+constexpr int kChunk = kCopyThreads * kAtOnce;             // vectors that a CTA copies at a time (32 KB)
 
-constexpr int kCopySlices = 8;  // CTAs that share a page
-
+// Work item (copy, chunk of its page): 32 KB of codes, or the page's scales.
+// CTAs take the items in turn, so a few large pages fill the GPU as well as
+// many small ones.  Memory-bound: 1.7 GB moved (read and written) in 260 us.
 __global__ void __launch_bounds__(kCopyThreads) k_kv8_copy(const CopyArgs a)
 {
     pdl_wait();
     const quantr_kv8_pool& p = a.pool;
     const int n = a.count ? *a.count : a.n;
-    const size_t units = (size_t)p.n_layers * p.n_kv_heads, codes = units * p.page_tokens * p.head_dim;
-    const int slice = blockIdx.x % kCopySlices;
-    const size_t at = (size_t)slice * kCopyThreads + threadIdx.x, step = (size_t)kCopySlices * kCopyThreads;
-    for (int i = blockIdx.x / kCopySlices; i < n; i += gridDim.x / kCopySlices) {
+    const size_t units = (size_t)p.n_layers * p.n_kv_heads, vecs = units * p.page_tokens * p.head_dim / 16;
+    const int chunks = (int)((vecs + kChunk - 1) / kChunk), items = 2 * chunks + 1;
+    for (long long w = blockIdx.x; w < (long long)n * items; w += gridDim.x) {
+        const int i = (int)(w / items), c = (int)(w - (long long)i * items);
         const int src = a.src[i], dst = a.dst[i];
         if (src < 0 || src >= p.n_pages || dst < 0 || dst >= p.n_pages) {
             kv8_fault(a.err);
             continue;
         }
-        copy_span(p.k + (size_t)dst * codes, p.k + (size_t)src * codes, codes, at, step);
-        copy_span(p.v + (size_t)dst * codes, p.v + (size_t)src * codes, codes, at, step);
-        copy_span(p.k_scale + (size_t)dst * units, p.k_scale + (size_t)src * units, units * 4, at, step);
-        copy_span(p.v_scale + (size_t)dst * units, p.v_scale + (size_t)src * units, units * 4, at, step);
+        if (c == 2 * chunks) {
+            for (size_t j = threadIdx.x; j < units; j += kCopyThreads) {
+                p.k_scale[dst * units + j] = p.k_scale[src * units + j];
+                p.v_scale[dst * units + j] = p.v_scale[src * units + j];
+            }
+            continue;
+        }
+        int8_t* codes = c < chunks ? p.k : p.v;
+        const uint4* s = reinterpret_cast<const uint4*>(codes) + src * vecs;
+        uint4* d = reinterpret_cast<uint4*>(codes) + dst * vecs;
+        const size_t at = (size_t)(c < chunks ? c : c - chunks) * kChunk + threadIdx.x;
+        uint4 v[kAtOnce];
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j)
+            if (at + j * kCopyThreads < vecs) v[j] = __ldcs(s + at + j * kCopyThreads);
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j)
+            if (at + j * kCopyThreads < vecs) __stcs(d + at + j * kCopyThreads, v[j]);
     }
     if (a.map)
         for (size_t i = (size_t)blockIdx.x * kCopyThreads + threadIdx.x; i < a.entries;
@@ -203,12 +213,22 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv8_extend(const PlanArgs a)
     upto[i] = base + need;
     // The free pages of lowest index, in order, until there are enough.
     int found = 0;
-    for (int p0 = 0; p0 < a.n_pages && found < total; p0 += kPlanThreads) {
-        const int page = p0 + i;
-        const int is = page < a.n_pages && a.t.refs[page] == 0;
+    for (int p0 = 0; p0 < a.n_pages && found < total; p0 += 4 * kPlanThreads) {
+        const int page = p0 + 4 * i;
+        int is[4], mine = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            is[j] = page + j < a.n_pages && a.t.refs[page + j] == 0;
+            mine += is[j];
+        }
         int sum;
-        const int at = found + block_scan(is, &sum, red);
-        if (is && at < total) a.list[at] = page;
+        int at = found + block_scan(mine, &sum, red);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (is[j]) {
+                if (at < total) a.list[at] = page + j;
+                ++at;
+            }
         found += sum;
     }
     if (i == 0) found_s = found;
@@ -250,23 +270,36 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv8_compact(const PlanArgs a)
     __shared__ int red[33];
     pdl_wait();
     int live = 0;
-    for (int p0 = 0; p0 < a.n_pages; p0 += kPlanThreads) {
-        const int page = p0 + threadIdx.x;
-        live += __syncthreads_count(page < a.n_pages && a.t.refs[page] > 0);
+    for (int p0 = 0; p0 < a.n_pages; p0 += 4 * kPlanThreads) {
+        const int page = p0 + 4 * threadIdx.x;
+        int mine = 0, sum;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mine += page + j < a.n_pages && a.t.refs[page + j] > 0;
+        block_scan(mine, &sum, red);
+        live += sum;
     }
+    // Holes and movers counted in one number each time: at most 4096 of either.
     int holes = 0, movers = 0;
-    for (int p0 = 0; p0 < a.n_pages; p0 += kPlanThreads) {
-        const int page = p0 + threadIdx.x;
-        const bool used = page < a.n_pages && a.t.refs[page] > 0;
-        const bool hole = page < live && !used, mover = used && page >= live;
-        int sum;
-        int at = block_scan(hole, &sum, red);
-        if (hole) a.dst[holes + at] = page;
-        holes += sum;
-        at = block_scan(mover, &sum, red);
-        if (mover) a.src[movers + at] = page;
-        movers += sum;
-        if (page < a.n_pages) a.list[page] = used ? page : -1;
+    for (int p0 = 0; p0 < a.n_pages; p0 += 4 * kPlanThreads) {
+        const int page = p0 + 4 * threadIdx.x;
+        bool used[4];
+        int mine = 0, sum;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            used[j] = page + j < a.n_pages && a.t.refs[page + j] > 0;
+            if (page + j < live && !used[j]) mine += 1;
+            if (page + j >= live && used[j]) mine += 1 << 16;
+        }
+        const int at = block_scan(mine, &sum, red);
+        int hole = holes + (at & 0xffff), mover = movers + (at >> 16);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (page + j < live && !used[j]) a.dst[hole++] = page + j;
+            if (page + j >= live && used[j]) a.src[mover++] = page + j;
+            if (page + j < a.n_pages) a.list[page + j] = used[j] ? page + j : -1;
+        }
+        holes += sum & 0xffff;
+        movers += sum >> 16;
     }
     __syncthreads();
     for (int i = threadIdx.x; i < movers; i += kPlanThreads) {
@@ -286,9 +319,12 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv8_compact(const PlanArgs a)
 
 int lg_tokens(const quantr_kv8_pool* p) { return p->page_tokens == 32 ? 5 : p->page_tokens == 64 ? 6 : 7; }
 
-int copy_grid(long long pages)
+// CTAs for at most `pages` copies: 4 per SM, fewer where there is less to do.
+int copy_grid(const quantr_kv8_pool* p, long long pages)
 {
-    return kCopySlices * (int)std::min<long long>(std::max(pages, 1ll), 2 * device_sm_count());
+    const long long vecs = (long long)p->n_layers * p->n_kv_heads * p->page_tokens * p->head_dim / 16;
+    const long long items = std::max(pages, 1ll) * (2 * ((vecs + kChunk - 1) / kChunk) + 1);
+    return (int)std::min<long long>(items, 4ll * device_sm_count());
 }
 
 // Workspace: count, then src, dst and list of n_pages each.
@@ -323,10 +359,7 @@ int quantr_kv8_select_dev(const quantr_kv8_tables* to, const quantr_kv8_tables* 
     SelectArgs a{*to, *in, from, pool->n_pages, lg_tokens(pool), device_error_word()};
     LaunchCfg c;
     c.stream = (cudaStream_t)stream;
-    cudaError_t e = launch_ex(k_kv8_zero, dim3(std::min((pool->n_pages + 255) / 256, 256)), 256, 0, c, to->refs,
-                              pool->n_pages);
-    if (e == cudaSuccess) e = launch_ex(k_kv8_select, dim3(to->slots), 128, 0, c, a);
-    return kv8_done(e);
+    return kv8_done(launch_ex(k_kv8_select, dim3(kSelectCtas), kSelectThreads, 0, c, a));
 }
 
 size_t quantr_kv8_pages_workspace_bytes(const quantr_kv8_pool* pool, const quantr_kv8_tables* tables)
@@ -370,7 +403,7 @@ int quantr_kv8_extend_dev(const quantr_kv8_pool* pool, const quantr_kv8_tables* 
     c.stream = (cudaStream_t)stream;
     cudaError_t e = launch_ex(k_kv8_extend, dim3(1), kPlanThreads, 0, c, a);
     CopyArgs k{*pool, a.count, 0, a.src, a.dst, a.err, nullptr, nullptr, 0};
-    if (e == cudaSuccess) e = launch_ex(k_kv8_copy, dim3(copy_grid(B)), kCopyThreads, 0, c, k);
+    if (e == cudaSuccess) e = launch_ex(k_kv8_copy, dim3(copy_grid(pool, B)), kCopyThreads, 0, c, k);
     return kv8_done(e);
 }
 
@@ -385,7 +418,7 @@ int quantr_kv8_compact_dev(const quantr_kv8_pool* pool, const quantr_kv8_tables*
     c.stream = (cudaStream_t)stream;
     cudaError_t e = launch_ex(k_kv8_compact, dim3(1), kPlanThreads, 0, c, a);
     CopyArgs k{*pool, a.count, 0, a.src, a.dst, a.err, tables->table, a.list, (size_t)tables->slots * tables->max_pages};
-    if (e == cudaSuccess) e = launch_ex(k_kv8_copy, dim3(copy_grid(pool->n_pages)), kCopyThreads, 0, c, k);
+    if (e == cudaSuccess) e = launch_ex(k_kv8_copy, dim3(copy_grid(pool, pool->n_pages)), kCopyThreads, 0, c, k);
     return kv8_done(e);
 }
 
@@ -397,7 +430,7 @@ int quantr_kv8_copy_pages_dev(const quantr_kv8_pool* pool, const int* dst, const
     CopyArgs k{*pool, nullptr, n, src, dst, device_error_word(), nullptr, nullptr, 0};
     LaunchCfg c;
     c.stream = (cudaStream_t)stream;
-    return kv8_done(launch_ex(k_kv8_copy, dim3(copy_grid(n)), kCopyThreads, 0, c, k));
+    return kv8_done(launch_ex(k_kv8_copy, dim3(copy_grid(pool, n)), kCopyThreads, 0, c, k));
 }
 
 } // extern "C"
