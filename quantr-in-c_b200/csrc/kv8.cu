@@ -9,24 +9,51 @@ namespace {
 
 // ----------------------------------------------------------------- append --
 
-constexpr int kVecs = 8;           // 16-byte vectors of a page that a thread holds
-constexpr int kAppendMax = 512;    // threads: 128 rows of 128 fp32 elements
+constexpr int kVecs = 4;           // 16-byte vectors of a page that a thread holds
+constexpr int kAppendMax = 1024;   // threads: 128 rows of 128 fp32 elements
 
-// Block maximum of non-negative floats; a NaN or infinity anywhere gives NaN.
-__device__ __forceinline__ float block_absmax(float m, bool bad, float* red)
+// Block maximum.
+__device__ __forceinline__ uint32_t block_max(uint32_t u, uint32_t* red)
 {
-    if (bad) m = __int_as_float(0x7fffffff);
-    // Non-negative floats (NaN above all) order like their bits.
-    uint32_t u = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
+    u = __reduce_max_sync(0xffffffffu, u);
     if (blockDim.x == 32) {
         __syncwarp();
-        return __uint_as_float(u);
+        return u;
     }
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = __uint_as_float(u);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = u;
     __syncthreads();
     u = 0;
-    for (int i = 0; i < (int)blockDim.x / 32; ++i) u = max(u, __float_as_uint(red[i]));
-    return __uint_as_float(u);
+    for (int i = 0; i < (int)blockDim.x / 32; ++i) u = max(u, red[i]);
+    return u;
+}
+
+// Magnitudes order like their bits, infinities and NaN above all others: the
+// largest of a vector's as an integer of the element's width, and its value
+// (NaN for either of those).
+template <typename T>
+__device__ __forceinline__ uint32_t vec_top(const uint4& v, uint32_t m)
+{
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) m = max(m, w[i] & 0x7fffffffu);
+        else m = __vmaxu2(m, w[i] & 0x7fff7fffu);  // two maxima, joined below
+    }
+    return m;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t top_bits(uint32_t m)
+{
+    return sizeof(T) == 4 ? m : max(m & 0xffffu, m >> 16);
+}
+template <typename T>
+__device__ __forceinline__ float top_value(uint32_t u)
+{
+    float f;
+    if constexpr (sizeof(T) == 4) f = __uint_as_float(u);
+    else if constexpr (std::is_same_v<T, __half>) f = __half2float(__ushort_as_half((unsigned short)u));
+    else f = __uint_as_float(u << 16);
+    return f <= 3.402823466e38f ? f : __int_as_float(0x7fffffff);
 }
 
 // Least j >= 0 with room * 2^j >= top (both finite, room >= 2^-120).
@@ -72,22 +99,16 @@ template <typename T>
 __global__ void __launch_bounds__(kAppendMax) k_kv8_append(const AppendArgs a)
 {
     constexpr int VE = 16 / sizeof(T);
-    __shared__ float red[kAppendMax / 32];
+    __shared__ uint32_t red[kAppendMax / 32];
     pdl_wait();
     const Kv8View& w = a.w;
     const int h = blockIdx.y, kv = blockIdx.z, b = blockIdx.x / a.span, threads = blockDim.x;
     const Kv8Seq s = kv8_seq(w, b);
     const PageRows r = page_rows(w, s, blockIdx.x % a.span);
     if (r.hi <= r.lo) return;
-    const int unit = kv8_unit(w, s, r.at, h);
-    if (unit < 0) return;
     const T* src = static_cast<const T*>(a.src[kv]) + r.row * a.ld[kv] + (long long)h * w.hd;
-    int8_t* page = (kv ? w.v : w.k) + (size_t)unit * w.P * w.hd;
-    float* scale = (kv ? w.vs : w.ks) + unit;
     // Vector q of the rows: row q / per_row, element (q % per_row) * VE.
     const int per_row = w.hd / VE, n = (r.hi - r.lo) * per_row, had = r.lo - (r.at << w.lgP);
-    const float old = had ? *scale : 0.0f;
-
     uint4 x[kVecs];
     const int row0 = threadIdx.x / per_row, col0 = threadIdx.x % per_row, drow = threads / per_row, dcol = threads % per_row;
     {
@@ -109,19 +130,15 @@ __global__ void __launch_bounds__(kAppendMax) k_kv8_append(const AppendArgs a)
             if (col >= per_row) col -= per_row, ++row;
         }
     }
-    float m = 0.0f;
-    bool bad = false;
+    const int unit = kv8_unit(w, s, r.at, h);
+    if (unit < 0) return;
+    int8_t* page = (kv ? w.v : w.k) + (size_t)unit * w.P * w.hd;
+    float* scale = (kv ? w.vs : w.ks) + unit;
+    const float old = had ? *scale : 0.0f;
+    uint32_t mb = 0;
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-        const T* e = reinterpret_cast<const T*>(&x[i]);
-#pragma unroll
-        for (int j = 0; j < VE; ++j) {
-            const float f = fabsf(to_f<T>(e[j]));
-            bad |= !(f <= 3.402823466e38f);
-            m = fmaxf(m, f);
-        }
-    }
-    m = block_absmax(m, bad, red);  // also: everybody has read the old scale
+    for (int i = 0; i < kVecs; ++i) mb = vec_top<T>(x[i], mb);
+    const float m = top_value<T>(block_max(top_bits<T>(mb), red));  // also: everybody has read the old scale
     float sc;
     int j = 0;
     if (!had) {
@@ -155,12 +172,14 @@ __global__ void __launch_bounds__(kAppendMax) k_kv8_append(const AppendArgs a)
         uint32_t c[VE / 4];
 #pragma unroll
         for (int g = 0; g < VE / 4; ++g) {
-            c[g] = 0;
+            // x/s is within 127 (and a few ulp) in magnitude: adding 1.5 * 2^23
+            // rounds it half to even into the low byte.
+            uint32_t v[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int v = sc == sc ? min(max(__float2int_rn(__fmul_rn(to_f<T>(e[4 * g + k]), inv)), -127), 127) : 0;
-                c[g] |= (uint32_t)(v & 255) << (8 * k);
-            }
+            for (int k = 0; k < 4; ++k)
+                v[k] = __float_as_uint(__fadd_rn(__fmul_rn(to_f<T>(e[4 * g + k]), inv), 12582912.0f));
+            c[g] = __byte_perm(__byte_perm(v[0], v[1], 0x0040), __byte_perm(v[2], v[3], 0x0040), 0x5410);
+            if (sc != sc) c[g] = 0;
         }
         if constexpr (VE == 4) *reinterpret_cast<uint32_t*>(dst + q * VE) = c[0];
         else *reinterpret_cast<uint2*>(dst + q * VE) = make_uint2(c[0], c[1]);
@@ -171,6 +190,7 @@ __global__ void __launch_bounds__(kAppendMax) k_kv8_append(const AppendArgs a)
 // ------------------------------------------------------------------- read --
 
 constexpr int kReadThreads = 256;
+constexpr int kReadAtOnce = 8;  // groups of four codes that a thread loads before it stores
 
 struct ReadArgs {
     Kv8View w;
@@ -204,13 +224,25 @@ __global__ void __launch_bounds__(kReadThreads) k_kv8_read(const ReadArgs a)
     const int n = (r.hi - r.lo) * q4;
     const int drow = kReadThreads / q4, dcol = kReadThreads % q4;
     int row = threadIdx.x / q4, col = threadIdx.x % q4;
-#pragma unroll 4
-    for (int g = threadIdx.x; g < n; g += kReadThreads) {
-        const char4 c = unit >= 0 ? reinterpret_cast<const char4*>(page)[g] : make_char4(0, 0, 0, 0);
-        const float x[4] = {c.x * sc, c.y * sc, c.z * sc, c.w * sc};
-        store4<T>(out + (r.row + row) * a.ld[kv] + col * 4, a.vec[kv], x);
-        row += drow, col += dcol;
-        if (col >= q4) col -= q4, ++row;
+    for (int g0 = threadIdx.x; g0 < n; g0 += kReadAtOnce * kReadThreads) {
+        uint32_t c[kReadAtOnce];
+#pragma unroll
+        for (int i = 0; i < kReadAtOnce; ++i) {
+            const int g = g0 + i * kReadThreads;
+            c[i] = unit >= 0 && g < n ? reinterpret_cast<const uint32_t*>(page)[g] : 0u;
+        }
+#pragma unroll
+        for (int i = 0; i < kReadAtOnce; ++i) {
+            // The bytes, offset by 128, as the low bits of 2^23.
+            const uint32_t u = c[i] ^ 0x80808080u;
+            float x[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                x[k] = (__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + k)) - 8388736.0f) * sc;
+            if (g0 + i * kReadThreads < n) store4<T>(out + (r.row + row) * a.ld[kv] + col * 4, a.vec[kv], x);
+            row += drow, col += dcol;
+            if (col >= q4) col -= q4, ++row;
+        }
     }
 }
 

@@ -102,10 +102,10 @@ struct CopyArgs {
     size_t entries;
 };
 
-constexpr int kAtOnce = 8;                                  // 16-byte loads in flight per thread
-constexpr int kChunk = kCopyThreads * kAtOnce;             // vectors that a CTA copies at a time (32 KB)
+constexpr int kAtOnce = 4;                      // 16-byte loads in flight per thread
+constexpr int kChunk = kCopyThreads * kAtOnce;  // vectors that a CTA copies at a time (16 KB)
 
-// Work item (copy, chunk of its page): 32 KB of codes, or the page's scales.
+// Work item (copy, chunk of its page): 16 KB of codes, or the page's scales.
 // CTAs take the items in turn, so a few large pages fill the GPU as well as
 // many small ones.  Memory-bound: 1.7 GB moved (read and written) in 260 us.
 __global__ void __launch_bounds__(kCopyThreads) k_kv8_copy(const CopyArgs a)
@@ -136,10 +136,10 @@ __global__ void __launch_bounds__(kCopyThreads) k_kv8_copy(const CopyArgs a)
         uint4 v[kAtOnce];
 #pragma unroll
         for (int j = 0; j < kAtOnce; ++j)
-            if (at + j * kCopyThreads < vecs) v[j] = __ldcs(s + at + j * kCopyThreads);
+            if (at + j * kCopyThreads < vecs) v[j] = s[at + j * kCopyThreads];
 #pragma unroll
         for (int j = 0; j < kAtOnce; ++j)
-            if (at + j * kCopyThreads < vecs) __stcs(d + at + j * kCopyThreads, v[j]);
+            if (at + j * kCopyThreads < vecs) d[at + j * kCopyThreads] = v[j];
     }
     if (a.map)
         for (size_t i = (size_t)blockIdx.x * kCopyThreads + threadIdx.x; i < a.entries;
@@ -169,7 +169,7 @@ struct PlanArgs {
 // One CTA, thread i plans sequence i.
 __global__ void __launch_bounds__(kPlanThreads) k_kv8_extend(const PlanArgs a)
 {
-    __shared__ int red[33], tails[kPlanThreads], upto[kPlanThreads];
+    __shared__ int red[33], tails[kPlanThreads];
     __shared__ int found_s;
     pdl_wait();
     const int i = threadIdx.x, P = 1 << a.lgP;
@@ -210,7 +210,6 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv8_extend(const PlanArgs a)
     const int need = ok ? (copied ? 1 : 0) + (new_pages - old_pages) : 0;
     int total;
     const int base = block_scan(need, &total, red);
-    upto[i] = base + need;
     // The free pages of lowest index, in order, until there are enough.
     int found = 0;
     for (int p0 = 0; p0 < a.n_pages && found < total; p0 += 4 * kPlanThreads) {
@@ -319,12 +318,14 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv8_compact(const PlanArgs a)
 
 int lg_tokens(const quantr_kv8_pool* p) { return p->page_tokens == 32 ? 5 : p->page_tokens == 64 ? 6 : 7; }
 
-// CTAs for at most `pages` copies: 4 per SM, fewer where there is less to do.
+// CTAs for at most `pages` copies: 32 per SM (several waves: their ends overlap
+// better than those of CTAs that stay; 4 per SM measured 7 % slower), fewer where
+// there is less to do.
 int copy_grid(const quantr_kv8_pool* p, long long pages)
 {
     const long long vecs = (long long)p->n_layers * p->n_kv_heads * p->page_tokens * p->head_dim / 16;
     const long long items = std::max(pages, 1ll) * (2 * ((vecs + kChunk - 1) / kChunk) + 1);
-    return (int)std::min<long long>(items, 4ll * device_sm_count());
+    return (int)std::min<long long>(items, 32ll * device_sm_count());
 }
 
 // Workspace: count, then src, dst and list of n_pages each.
