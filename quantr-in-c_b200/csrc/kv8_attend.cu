@@ -381,7 +381,7 @@ __device__ __forceinline__ float digits_value(const int (&c)[DG][C], int r)
 }
 
 template <typename T, int RT, int HDW>
-__global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const __grid_constant__ AttendParams p)
+__global__ void __launch_bounds__(kThreads, 2) k_kv8_attend(const __grid_constant__ AttendParams p)
 {
     constexpr int DG = digits<T>;
     constexpr int N = Shape<DG, RT>::N;
@@ -1005,10 +1005,13 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 2 : 1) k_kv8_attend(const
 
 // --------------------------------------------------------------- host side --
 
+// Rows of a row tile: a sequence's rows (tokens x query heads of a KV head) if
+// they fit, else 16.  32 measured slower (64-token chunks 83 us against 67, 512
+// tokens 320 against 265): its registers leave one CTA per SM.
 int pick_rt(const quantr_kv8_batch* b, int G)
 {
     const long long rows = (long long)b->max_rows * G;
-    return rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
+    return rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
 }
 
 struct Plan {
@@ -1082,8 +1085,7 @@ cudaError_t run_rt(int rt, AttendParams& p, const quantr_kv8_pool* pool, void* w
     switch (rt) {
     case 4: return run<T, 4, HDW>(p, pool, ws, c);
     case 8: return run<T, 8, HDW>(p, pool, ws, c);
-    case 16: return run<T, 16, HDW>(p, pool, ws, c);
-    default: return run<T, 32, HDW>(p, pool, ws, c);
+    default: return run<T, 16, HDW>(p, pool, ws, c);
     }
 }
 
