@@ -171,6 +171,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv8_extend(const PlanArgs a)
 {
     __shared__ int red[33], tails[kPlanThreads];
     __shared__ int found_s;
+    __shared__ bool failed[kPlanThreads];
     pdl_wait();
     const int i = threadIdx.x, P = 1 << a.lgP;
     int slot = -1, len = 0, n = 0, tail = -1;
@@ -232,7 +233,16 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv8_extend(const PlanArgs a)
     }
     if (i == 0) found_s = found;
     __syncthreads();
-    if (ok && base + need > found_s) {
+    // Out of pages: for this sequence and for every later one that needs one.
+    // Who would have kept a shared page as the last of its holders needs one,
+    // too, if one of the others got no copy.
+    const bool late = ok && need > 0 && base + need > found_s;
+    failed[i] = late;
+    __syncthreads();
+    bool left = false;
+    if (ok && tail >= 0 && !copied)
+        for (int j = 0; j < i; ++j) left |= tails[j] == tail && failed[j];
+    if (late || left) {
         kv8_fault(a.err);
         ok = false;
     }

@@ -94,7 +94,8 @@ __device__ __forceinline__ Sums join(Sums a, Sums b, float c)
     Sums r;
     r.m = fmaxf(a.m, b.m);
     if (r.m == -INFINITY) return {r.m, a.s + b.s, a.e + b.e};
-    const float da = (a.m - r.m) * c, db = (b.m - r.m) * c;
+    // (2^-200 is 0, and bounded it makes no 0 * -inf; NaN stays.)
+    const float da = lp_max_nan((a.m - r.m) * c, -200.0f), db = lp_max_nan((b.m - r.m) * c, -200.0f);
     const float fa = lp_ex2(da), fb = lp_ex2(db);
     r.s = a.s * fa + b.s * fb;
     r.e = (a.m == -INFINITY ? a.s : fmaf(a.s, da, a.e) * fa) + (b.m == -INFINITY ? b.s : fmaf(b.s, db, b.e) * fb);
@@ -318,7 +319,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LpArgs a)
     auto raise = [&](float mt) {
         if (mt > st.m) {
             if (st.m > -INFINITY) {
-                const float d = (st.m - mt) * a.c, r = lp_ex2(d);
+                const float d = lp_max_nan((st.m - mt) * a.c, -200.0f), r = lp_ex2(d);
                 st.e = fmaf(st.s, d, st.e) * r;
                 st.s *= r;
             }
