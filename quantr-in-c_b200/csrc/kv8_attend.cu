@@ -323,7 +323,7 @@ struct Shape {
 struct Bars {
     uint64_t kfull[kMaxStages], kempty[kMaxStages], vfull[kMaxStages], vempty[kMaxStages];
     uint64_t sfull[2], sempty[2], pfull[2], ofull[2], joined[2];
-    uint64_t mfull[kMeta], segfull[kMeta], qfull, pmax[2][2], jdone, jlast;
+    uint64_t mfull[kMeta], segfull[kMeta], qfull, jdone, jlast;
 };
 
 struct Meta {
@@ -422,7 +422,6 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_attend(const __grid_constan
             mbar_init(&br.segfull[i], 1);
         }
         mbar_init(&br.qfull, 4);
-        for (int i = 0; i < 4; ++i) mbar_init(&br.pmax[i >> 1][i & 1], 1 << (lgP - 5));
         mbar_init(&br.jdone, 4);
         mbar_init(&br.jlast, 1);
         z.abort = 0;
@@ -613,9 +612,24 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_attend(const __grid_constan
         };
         float qx[kRows][4];
         Seg k;
-        bool ok = true, more = next_seg(k);
+        // Whether all warps of the page say so.  A named barrier costs a tenth of
+        // an mbarrier's round trip (25 and 300 cycles), but its wait has no
+        // limit: these warps therefore meet the same number of times whatever
+        // happens, and leave their loops together, on its answer.
+        auto all_of = [&](bool mine) -> bool {
+            if (lgP == 5) return mine;
+            uint32_t all;
+            asm volatile(
+                "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %3, 0;\n\t"
+                "bar.red.and.pred p, %1, %2, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                : "=r"(all)
+                : "r"(lgP == 6 ? 1 + (warp >> 1) : 1), "r"(lgP == 6 ? 64 : 128), "r"((uint32_t)mine)
+                : "memory");
+            return all != 0;
+        };
+        bool ok = true, more = all_of(next_seg(k));
         if (more) load_q(k, qx);
-        while (ok && more) {
+        while (more) {
             // The row tile's query rows as digits.  Its last product has read
             // the old ones (its scores have arrived).
             const int base_pos = k.len - k.n, sg = seg & 1;
@@ -661,7 +675,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_attend(const __grid_constan
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(&br.qfull);
-            if (!(ok = warp_wait(&br.qfull, seg++ & 1, err, abort))) break;
+            if (!(ok = all_of(warp_wait(&br.qfull, seg++ & 1, err, abort)))) break;
             const int pos_lo = z.pos[sg][0], pos_hi = z.pos[sg][RT - 1];
 
             const int t0 = k.t0, t1 = k.t1;
@@ -671,8 +685,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_attend(const __grid_constan
                     more = next_seg(k);
                     if (more) load_q(k, qx);
                 }
-                ok = warp_wait(&br.mfull[mt], mu & 1, err, abort) && warp_wait(&br.sfull[sb], su & 1, err, abort);
-                if (!ok) break;
+                ok = ok && warp_wait(&br.mfull[mt], mu & 1, err, abort) && warp_wait(&br.sfull[sb], su & 1, err, abort);
+                if (lgP == 5 && !ok) break;
                 const Meta& m = z.meta[mt];
                 const float ks = m.ks[page];
                 const int valid = m.valid;
@@ -710,25 +724,23 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_attend(const __grid_constan
 #pragma unroll
                 for (int r = 0; r < RT; ++r) mx[r] = warp_max_nan(x[r]);
                 if (lgP > 5) {  // the page spans several warps
-                    const int w0 = lgP == 6 ? warp & 2 : 0, wn = 1 << (lgP - 5);
-                    if (lane == 0) {
-                        store_rows<RT>(z.wmax[pb][warp], mx);
-                        mbar_arrive(&br.pmax[pb][w0 >> 1]);
-                    }
-                    if (!(ok = warp_wait(&br.pmax[pb][w0 >> 1], pu & 1, err, abort))) break;
-#pragma unroll 1
-                    for (int w = w0; w < w0 + wn; ++w) {
+                    const int wn = 1 << (lgP - 5);
+                    if (lane == 0) store_rows<RT>(z.wmax[pb][warp], mx);
+                    if (!(ok = all_of(ok))) break;
 #pragma unroll
-                        for (int r = 0; r < RT; r += 4) {
-                            const float4 v = *reinterpret_cast<const float4*>(&z.wmax[pb][w][r]);
-                            mx[r] = max_nan(mx[r], v.x), mx[r + 1] = max_nan(mx[r + 1], v.y);
-                            mx[r + 2] = max_nan(mx[r + 2], v.z), mx[r + 3] = max_nan(mx[r + 3], v.w);
-                        }
+                    for (int i = 1; i < 4; ++i) {
+                        if (i >= wn) break;
+                        const float* other = z.wmax[pb][(warp & ~(wn - 1)) | ((warp + i) & (wn - 1))];
+                        float v[RT];
+                        load_rows<RT>(other, v);
+#pragma unroll
+                        for (int r = 0; r < RT; ++r) mx[r] = max_nan(mx[r], v[r]);
                     }
                 }
                 // The tile before the last is joined: its weights were used and
                 // its maxima read.
-                if (pu > 0 && !(ok = warp_wait(&br.joined[pb], (pu - 1) & 1, err, abort))) break;
+                // (A warp that gave up here says so at its next all_of.)
+                if (pu > 0) ok = warp_wait(&br.joined[pb], (pu - 1) & 1, err, abort);
                 float sum[RT];
                 uint8_t* pt = psm + pb * kPBytes + (tid & 15);
 #pragma unroll
@@ -764,6 +776,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_attend(const __grid_constan
                 if (++pb == 2) pb = 0, ++pu;
                 if (++mt == kMeta) mt = 0, ++mu;
             }
+            more = all_of(more && ok);
         }
     } else if (warp < 8) {
         // ------------------------------------------------------------ join --
