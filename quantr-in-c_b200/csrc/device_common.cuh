@@ -226,11 +226,9 @@ __device__ __forceinline__ void st_remote(uint32_t a, unsigned long long v)
 {
     asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(v) : "memory");
 }
-__device__ __forceinline__ int add_remote(uint32_t a, int v)
+__device__ __forceinline__ void st_remote(uint32_t a, int v)
 {
-    int r;
-    asm volatile("atom.shared::cluster.add.s32 %0, [%1], %2;" : "=r"(r) : "r"(a), "r"(v) : "memory");
-    return r;
+    asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
 }
 
 // dp4a with unsigned bytes in `a` and signed bytes in `b`.

@@ -30,7 +30,7 @@ constexpr int kMaxTop = 64;
 constexpr int kGroups = 32;       // groups of a thread's tiles, at most
 constexpr int kMaxHeads = 128;    // values that the threshold is chosen from
 constexpr int kHits = 1024;       // groups that are read again
-constexpr int kCap = 1024;        // candidates that are ranked against each other
+constexpr int kCap = 512;         // candidates that are ranked against each other
 constexpr int kMaxSplit = 8;      // CTAs of a row: one cluster
 
 typedef unsigned long long u64;
@@ -39,7 +39,8 @@ struct LpArgs {
     const void* x;
     long long ldl;
     int rows, V, k, split;
-    float inv_t, c;  // 1/temperature, and times log2(e)
+    double inv_t;  // 1 / temperature
+    float c;       // times log2(e)
     const int* token;
     float* logprob;
     float* entropy;
@@ -88,18 +89,30 @@ struct Sums {
     float m, s, e;
 };
 
-// Both about the larger maximum.
-__device__ __forceinline__ Sums join(Sums a, Sums b, float c)
+// Sums of more than one thread are held in 64 bits: a row's rounding is then
+// that of its results, for a few operations per row.
+struct WideSums {
+    float m;
+    double s, e;
+};
+
+// The warp's sums about their largest maximum; in all lanes.
+__device__ __forceinline__ WideSums join_warp(WideSums a, float c)
 {
-    Sums r;
-    r.m = fmaxf(a.m, b.m);
-    if (r.m == -INFINITY) return {r.m, a.s + b.s, a.e + b.e};
-    // (2^-200 is 0, and bounded it makes no 0 * -inf; NaN stays.)
-    const float da = lp_max_nan((a.m - r.m) * c, -200.0f), db = lp_max_nan((b.m - r.m) * c, -200.0f);
-    const float fa = lp_ex2(da), fb = lp_ex2(db);
-    r.s = a.s * fa + b.s * fb;
-    r.e = (a.m == -INFINITY ? a.s : fmaf(a.s, da, a.e) * fa) + (b.m == -INFINITY ? b.s : fmaf(b.s, db, b.e) * fb);
-    return r;
+    const float m = warp_max(a.m);
+    if (m > -INFINITY) {
+        // (2^-200 is 0, and bounded it makes no 0 * -inf; NaN stays.)
+        const float d = lp_max_nan((a.m - m) * c, -200.0f), f = lp_ex2(d);
+        a.e = (a.e + a.s * d) * f;
+        a.s *= f;
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) {
+        a.s += __shfl_xor_sync(~0u, a.s, d);
+        a.e += __shfl_xor_sync(~0u, a.e, d);
+    }
+    a.m = m;
+    return a;
 }
 
 template <typename T>
@@ -211,13 +224,15 @@ __device__ __forceinline__ float vec_max(const uint4& v)
     }
 }
 
-struct LpShared {
-    u64 buf[kCap];  // of the row's first CTA, as are count and part
+struct alignas(16) LpShared {
+    float heads[kMaxHeads];  // every warp's largest thread maxima, of the whole row
+    u64 slot[kCap];          // of the row's first CTA, as are found and part: a stretch for each CTA's candidates
+    u64 buf[kCap];
     u64 tops[kMaxTop];
     u64 best[kLpWarps];
-    float heads[kMaxHeads];  // every warp's largest thread maxima, of the whole row
     float low;
-    Sums part[kMaxSplit], sums[kLpWarps];
+    WideSums part[kMaxSplit * kLpWarps];
+    int found[kMaxSplit];
     int count, hits;
     uint16_t hit[kHits];  // group * threads + thread
     float group_max[1];   // [group][thread]
@@ -294,10 +309,19 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LpArgs a)
     LpShared& z = *reinterpret_cast<LpShared*>(raw);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) z.count = z.hits = 0, z.low = -INFINITY;
+    if (tid < kMaxHeads) z.heads[tid] = -INFINITY;
+    if (tid < kMaxSplit * kLpWarps) z.part[tid] = {-INFINITY, 0.0, 0.0};
     cluster_arrive();  // every CTA of the cluster has begun, and zeroed its counts: waited for before the first remote access
     pdl_wait();
     const int row = blockIdx.x / a.split, slice = blockIdx.x % a.split;
     const T* x = static_cast<const T*>(a.x) + row * a.ldl;
+    // The given token and its logit, two dependent loads that the pass hides.
+    int token = -1;
+    float token_x = 0.0f;
+    if (tid == 0 && slice == 0 && a.logprob) {
+        token = a.token[row];
+        if (token >= 0 && token < a.V) token_x = to_f<T>(x[token]);
+    }
     // Elements before the first 16-byte boundary, whole vectors, the rest.
     const int head = min(a.V, (int)(((16 - ((uintptr_t)x & 15)) & 15) / sizeof(T)));
     const int nvec = (a.V - head) / VE, tail = a.V - head - nvec * VE;
@@ -416,16 +440,6 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LpArgs a)
     // Warps that the threshold looks at: all of them, or those that a short row
     // fills (a split row's slices are long).
     const int nw = a.split > 1 ? kLpWarps : max(1, min(kLpWarps, nvec / 32));
-    // The row's sums: over the warp, the CTA, the cluster.
-    Sums mine = st;
-    for (int d = 16; d; d >>= 1) {
-        Sums o;
-        o.m = __shfl_xor_sync(~0u, mine.m, d);
-        o.s = __shfl_xor_sync(~0u, mine.s, d);
-        o.e = __shfl_xor_sync(~0u, mine.e, d);
-        mine = lane & d ? join(o, mine, a.c) : join(mine, o, a.c);  // the same operands in the same order on both lanes
-    }
-    if (lane == 0) z.sums[warp] = mine;
     // Each warp's `per_warp` largest thread maxima, told to every CTA of the row.
     const int heads = nw * a.split, per_warp = a.k ? min((a.k + heads - 1) / heads + 1, min(32, kMaxHeads / heads)) : 0;
     float y = st.m, head_val = -INFINITY;
@@ -436,17 +450,16 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LpArgs a)
         if (lane == __ffs(who) - 1) y = -INFINITY;
         if (lane == i) head_val = top;
     }
-    __syncthreads();
+    const WideSums mine = join_warp({st.m, st.s, st.e}, a.c);
     cluster_wait();
     if (warp < nw && lane < per_warp)
         for (int r = 0; r < a.split; ++r)
             st_remote(remote_of(&z.heads[(slice * nw + warp) * per_warp + lane], r), head_val);
-    if (tid == 0) {
-        Sums t = z.sums[0];
-        for (int w = 1; w < kLpWarps; ++w) t = join(t, z.sums[w], a.c);
-        st_remote(remote_of(&z.part[slice].m, 0), t.m);
-        st_remote(remote_of(&z.part[slice].s, 0), t.s);
-        st_remote(remote_of(&z.part[slice].e, 0), t.e);
+    if (lane == 0) {
+        const uint32_t to = remote_of(&z.part[slice * kLpWarps + warp], 0);
+        st_remote(to, mine.m);
+        st_remote(to + 8, (u64)__double_as_longlong(mine.s));
+        st_remote(to + 16, (u64)__double_as_longlong(mine.e));
     }
     __syncwarp();
     cluster_arrive();
@@ -457,23 +470,24 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LpArgs a)
         const int n = heads * per_warp;
         if (tid < n) {
             const float v = z.heads[tid];
-            int rank = 0;
-#pragma unroll 8
-            for (int i = 0; i < n; ++i) rank += z.heads[i] > v || (z.heads[i] == v && i < tid);
-            if (rank == a.k - 1) z.low = v;
+            int above = 0, reach = 0;
+#pragma unroll 4
+            for (int i = 0; i < n; i += 4) {
+                const float4 h = *reinterpret_cast<const float4*>(&z.heads[i]);
+                above += (h.x > v) + (h.y > v) + (h.z > v) + (h.w > v);
+                reach += (h.x >= v) + (h.y >= v) + (h.z >= v) + (h.w >= v);
+            }
+            if (above < a.k && a.k <= reach) z.low = v;
         }
         __syncthreads();
         const float low = z.low;
-        const uint32_t count = remote_of(&z.count, 0), buf = remote_of(z.buf, 0);
+        // Candidates go to this CTA's stretch of the first CTA's slots.
+        const int room = kCap / a.split;
+        const uint32_t slots = remote_of(&z.slot[slice * room], 0);
         auto push = [&](float y, int id) {
             if (!(y >= low && y > -INFINITY)) return;
-            if (a.split == 1) {
-                const int i = atomicAdd(&z.count, 1);
-                if (i < kCap) z.buf[i] = lp_key(y, id);
-            } else {
-                const int i = add_remote(count, 1);
-                if (i < kCap) st_remote(buf + 8 * i, lp_key(y, id));
-            }
+            const int i = atomicAdd(&z.count, 1);
+            if (i < room) st_remote(slots + 8 * i, lp_key(y, id));
         };
         if (st.m >= low && st.m > -INFINITY)
             for (int q = 0; q < group; ++q)
@@ -483,7 +497,6 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LpArgs a)
                 }
         __syncthreads();
         const int hits = min(z.hits, kHits);
-        if (z.hits > kHits && tid == 0) add_remote(count, kCap + 1);
         for (int i = tid; i < hits * kVecs * gt; i += kLpThreads) {
             // Vector i % (kVecs * gt) of the group.
             const int h = z.hit[i / (kVecs * gt)], j = i % (kVecs * gt), th = h % kLpThreads;
@@ -500,41 +513,50 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LpArgs a)
                 push(to_f<T>(x[id]), id);
             }
         }
+        __syncthreads();
+        if (tid == 0) st_remote(remote_of(&z.found[slice], 0), z.hits > kHits || z.count > room ? -1 : z.count);
         __syncwarp();
         cluster_arrive();
         if (slice) return;  // nobody reads this CTA's shared memory any more
         cluster_wait();
-        if (z.count <= kCap) {
-            rank_keys(z, z.count, a.k);
-        } else {
-            crowded<T>(a, z, x, low);
+        // The stretches, one behind the other.
+        int total = 0;
+        bool fits = true;
+        for (int r = 0; r < a.split; ++r) {
+            const int m = z.found[r];
+            fits &= m >= 0;
+            for (int i = tid; i < m; i += kLpThreads) z.buf[total + i] = z.slot[r * room + i];
+            total += max(m, 0);
         }
+        __syncthreads();
+        if (fits) rank_keys(z, total, a.k);
+        else crowded<T>(a, z, x, low);
     } else if (slice) {
         return;
     }
-    st = z.part[0];
-    for (int i = 1; i < a.split; ++i) st = join(st, z.part[i], a.c);
-    constexpr float ln2 = 0.693147180559945f;
-    const float l2 = log2f(st.s);
-    const bool bad = st.s != st.s || st.m == INFINITY;
-    float lse = fmaf(l2, ln2, st.m * a.inv_t), ent = (l2 - st.e / st.s) * ln2;
-    if (st.m == -INFINITY) lse = -INFINITY, ent = 0.0f;
+    // The row's sums, from every warp's (64 places, the others empty), in each
+    // warp: the alternatives need lse.
+    const WideSums t = join_warp(z.part[lane], a.c), u = join_warp(z.part[32 + lane], a.c);
+    const WideSums sum = join_warp(lane == 0 ? t : lane == 1 ? u : WideSums{-INFINITY, 0.0, 0.0}, a.c);
+    const double ls = log(sum.s);
+    const bool bad = sum.s != sum.s || sum.m == INFINITY;
+    double lse = sum.m * a.inv_t + ls, ent = ls - sum.e / sum.s * 0.6931471805599453;
+    if (sum.m == -INFINITY) lse = -INFINITY, ent = 0.0;
     if (bad) lse = ent = NAN;
     if (tid == 0) {
-        if (a.lse) a.lse[row] = lse;
-        if (a.entropy) a.entropy[row] = ent;
+        if (a.lse) a.lse[row] = (float)lse;
+        if (a.entropy) a.entropy[row] = (float)ent;
         if (a.logprob) {
-            const int t = a.token[row];
-            float lp = 0.0f;
-            if (t >= 0 && t < a.V) lp = lse == -INFINITY ? -INFINITY : to_f<T>(x[t]) * a.inv_t - lse;
-            else if (t != -1) lp = NAN;
-            a.logprob[row] = lp;
+            double lp = 0.0;
+            if (token >= 0 && token < a.V) lp = lse == -INFINITY ? -INFINITY : token_x * a.inv_t - lse;
+            else if (token != -1) lp = NAN;
+            a.logprob[row] = (float)lp;
         }
     }
     for (int i = tid; i < a.k; i += kLpThreads) {
         const u64 key = z.tops[i];
         if (a.top_id) a.top_id[(size_t)row * a.k + i] = key ? (int)~(uint32_t)key : -1;
-        if (a.top_lp) a.top_lp[(size_t)row * a.k + i] = bad ? NAN : key ? lp_value(key) * a.inv_t - lse : -INFINITY;
+        if (a.top_lp) a.top_lp[(size_t)row * a.k + i] = bad ? NAN : key ? (float)(lp_value(key) * a.inv_t - lse) : -INFINITY;
     }
 }
 
@@ -574,7 +596,7 @@ int quantr_logprobs_dev(const void* x, long long ldl, uint32_t type, int rows, i
     LpArgs a{};
     a.x = x, a.ldl = ldl, a.rows = rows, a.V = vocab, a.k = k, a.split = lp_split(rows, vocab);
     if ((long long)rows * a.split > 0x7fffffffll) return QUANTR_ERR_TOO_LARGE;
-    a.inv_t = (float)(1.0 / (double)temperature);
+    a.inv_t = 1.0 / (double)temperature;
     a.c = (float)(1.4426950408889634 / (double)temperature);
     a.token = token, a.logprob = logprob, a.entropy = entropy, a.lse = lse, a.top_id = top_id, a.top_lp = top_logprob;
     LaunchCfg c;
