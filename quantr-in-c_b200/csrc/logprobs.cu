@@ -441,7 +441,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LpArgs a)
     // fills (a split row's slices are long).
     const int nw = a.split > 1 ? kLpWarps : max(1, min(kLpWarps, nvec / 32));
     // Each warp's `per_warp` largest thread maxima, told to every CTA of the row.
-    const int heads = nw * a.split, per_warp = a.k ? min((a.k + heads - 1) / heads + 1, min(32, kMaxHeads / heads)) : 0;
+    const int heads = nw * a.split, per_warp = a.k ? min((2 * a.k + heads - 1) / heads, min(32, kMaxHeads / heads)) : 0;
     float y = st.m, head_val = -INFINITY;
     if (a.k && left < gt) z.group_max[group++ * kLpThreads + tid] = gmax;
     for (int i = 0; i < per_warp && warp < nw; ++i) {
@@ -519,15 +519,18 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LpArgs a)
         cluster_arrive();
         if (slice) return;  // nobody reads this CTA's shared memory any more
         cluster_wait();
-        // The stretches, one behind the other.
-        int total = 0;
+        // The stretches, one behind the other: warp r moves CTA r's.
+        int total = 0, at = 0;
         bool fits = true;
-        for (int r = 0; r < a.split; ++r) {
-            const int m = z.found[r];
+#pragma unroll
+        for (int r = 0; r < kMaxSplit; ++r) {
+            const int m = r < a.split ? z.found[r] : 0;
             fits &= m >= 0;
-            for (int i = tid; i < m; i += kLpThreads) z.buf[total + i] = z.slot[r * room + i];
-            total += max(m, 0);
+            if (r < warp) at += m;
+            total += m;
         }
+        if (fits && warp < a.split)
+            for (int i = lane; i < z.found[warp]; i += 32) z.buf[at + i] = z.slot[warp * room + i];
         __syncthreads();
         if (fits) rank_keys(z, total, a.k);
         else crowded<T>(a, z, x, low);
@@ -536,8 +539,15 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LpArgs a)
     }
     // The row's sums, from every warp's (64 places, the others empty), in each
     // warp: the alternatives need lse.
-    const WideSums t = join_warp(z.part[lane], a.c), u = join_warp(z.part[32 + lane], a.c);
-    const WideSums sum = join_warp(lane == 0 ? t : lane == 1 ? u : WideSums{-INFINITY, 0.0, 0.0}, a.c);
+    WideSums sum = z.part[lane];
+    if (a.split * kLpWarps > 32) {
+        const WideSums u = z.part[32 + lane];
+        const bool up = u.m > sum.m;
+        const WideSums &hi = up ? u : sum, &lo = up ? sum : u;
+        const float d = hi.m > -INFINITY ? lp_max_nan((lo.m - hi.m) * a.c, -200.0f) : 0.0f, f = lp_ex2(d);
+        sum = {hi.m, hi.s + lo.s * f, hi.e + (lo.e + lo.s * d) * f};
+    }
+    sum = join_warp(sum, a.c);
     const double ls = log(sum.s);
     const bool bad = sum.s != sum.s || sum.m == INFINITY;
     double lse = sum.m * a.inv_t + ls, ent = ls - sum.e / sum.s * 0.6931471805599453;
