@@ -208,6 +208,14 @@ __device__ __forceinline__ void walk_enter(const AttendParams& p, Walk& k)
     k.seg.c1 = (item0 + k.nt - 1) / k.share;
 }
 
+// a / b of small non-negative numbers by the approximate reciprocal: with
+// a < 2^21 its error is less than the half that is added.
+__device__ __forceinline__ int quotient(int a, int b)
+{
+    if (a >= 1 << 21) return a / b;
+    return (int)__fdividef((float)a + 0.5f, (float)b);
+}
+
 // This CTA's part of the work and its first segment.  Two ways to share it out:
 //   by row tiles, where there are no more of them than CTAs and their lengths
 //   differ little: a row tile has `per` CTAs, each with one run of its tiles
@@ -221,38 +229,58 @@ __device__ __forceinline__ void walk_begin(const AttendParams& p, Walk& k)
     int tiles = 0, items = 0, longest = 0;
     constexpr int kKept = 4;
     int nts[kKept], its[kKept];  // of the first 128 sequences, read at once and kept
-    auto look = [&](int b0, int& nt, int& it) {
+    // (Faults are reported when a sequence's turn comes, not here: nothing may
+    // stand between these loads.)
+    auto load = [&](int b0, int& n, int& len) {
+        const int b = b0 + lane;
+        n = len = 0;
+        if (b >= p.w.B) return;
+        const int slot = p.w.slot ? p.w.slot[b] : b;
+        n = p.w.start ? min(max(p.w.start[b + 1] - p.w.start[b], 0), p.w.max_rows) : p.w.max_rows;
+        if (slot >= 0 && slot < p.w.slots) len = p.w.lens[slot];
+    };
+    auto look = [&](int n, int len, int& nt, int& it) {
         int nrt, tlo;
-        nt = it = 0;
-        if (b0 + lane < p.w.B) {
-            const Kv8Seq s = kv8_seq(p.w, b0 + lane);
-            const int all = seq_tiles<RT>(p, s, nrt, nt, tlo);
-            it = all ? p.w.KV * nrt : 0;
-        }
+        Kv8Seq s;
+        s.n = n, s.len = len;
+        seq_tiles<RT>(p, s, nrt, nt, tlo);
+        it = p.w.KV * nrt;
     };
     auto add = [&](int nt, int it) {
         tiles += nt * it;
         items += it;
         longest = max(longest, it ? nt : 0);
     };
+    {
+        int n[kKept], len[kKept];
 #pragma unroll
-    for (int i = 0; i < kKept; ++i) look(32 * i, nts[i], its[i]);
+        for (int i = 0; i < kKept; ++i) load(32 * i, n[i], len[i]);
 #pragma unroll
-    for (int i = 0; i < kKept; ++i) add(nts[i], its[i]);
+        for (int i = 0; i < kKept; ++i) {
+            look(n[i], len[i], nts[i], its[i]);
+            add(nts[i], its[i]);
+        }
+    }
 #pragma unroll 1
     for (int b0 = 32 * kKept; b0 < p.w.B; b0 += 32) {
-        int nt, it;
-        look(b0, nt, it);
+        int n, len, nt, it;
+        load(b0, n, len);
+        look(n, len, nt, it);
         add(nt, it);
     }
     tiles = __reduce_add_sync(~0u, tiles);
     items = __reduce_add_sync(~0u, items);
     longest = __reduce_max_sync(~0u, longest);
-    k.share = (tiles + ctas - 1) / max(ctas, 1);
-    const int per = items > 0 ? ctas / items : 0;
-    const bool by_items = per > 0 && (longest + per - 1) / per <= k.share + kSlack;
-    k.pos = by_items ? me / per : min((int)min((long long)k.share * me, 0x7fffffffll), tiles);
-    k.end = by_items ? items : min(k.pos + k.share, tiles);
+    const int per = items > 0 && items <= ctas ? quotient(ctas, items) : 0;
+    const bool by_items = per > 0 && (float)longest <= per * ((float)tiles / ctas + kSlack + 1);
+    if (by_items) {
+        k.pos = quotient(me, per);
+        k.end = items;
+    } else {
+        k.share = (tiles + ctas - 1) / ctas;
+        k.pos = (int)min((long long)k.share * me, (long long)tiles);
+        k.end = min(k.pos + k.share, tiles);
+    }
     k.first = k.cnt = 0;
     k.b = -1;
     // The 32 sequences that pos lies in, and the one of them.
@@ -262,7 +290,11 @@ __device__ __forceinline__ void walk_begin(const AttendParams& p, Walk& k)
 #pragma unroll
         for (int i = 1; i < kKept; ++i)
             if (b0 == 32 * i) nt = nts[i], it = its[i];
-        if (b0 >= 32 * kKept) look(b0, nt, it);
+        if (b0 >= 32 * kKept) {
+            int n, len;
+            load(b0, n, len);
+            look(n, len, nt, it);
+        }
         const int c = by_items ? it : nt * it;
         int x = c;
 #pragma unroll
@@ -287,14 +319,14 @@ __device__ __forceinline__ void walk_begin(const AttendParams& p, Walk& k)
         k.s = kv8_seq(p.w, k.b);
         seq_tiles<RT>(p, k.s, k.nrt, k.nt, k.tlo);
         const int item = k.pos - k.first;
-        const int run = max((k.nt + per - 1) / per, (int)ceilf(sqrtf((float)k.nt * (1.0f / 12.0f))));
-        k.seg.h = item / k.nrt;
+        const int run = max(quotient(k.nt + per - 1, per), (int)ceilf(sqrtf((float)k.nt * (1.0f / 12.0f))));
+        k.seg.h = quotient(item, k.nrt);
         k.seg.rt = item - k.seg.h * k.nrt;
         k.seg.row0 = k.s.row0, k.seg.n = k.s.n, k.seg.len = k.s.len;
         k.seg.t0 = min(part * run, k.nt) + k.tlo;
         k.seg.t1 = min(part * run + run, k.nt) + k.tlo;
         k.seg.c0 = k.pos * per;
-        k.seg.c1 = k.seg.c0 + (k.nt + run - 1) / run - 1;
+        k.seg.c1 = k.seg.c0 + quotient(k.nt + run - 1, run) - 1;
         k.pos = k.end = 0;  // and no more after it
         return;
     }
@@ -460,7 +492,6 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_attend(const __grid_constan
         int st = 0, use = 0, mt = 0;
         struct Batch {
             int tiles, unit, have;
-            float ks, vs;
         };
         Walk k;
         walk_begin<RT>(p, k);
@@ -474,27 +505,28 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_attend(const __grid_constan
         publish();
         int at_t = k.seg.t0;
         auto fetch = [&]() -> Batch {
-            Batch f{0, 0, 0, 0.0f, 0.0f};
+            Batch f{0, 0, 0};
+            if (at_t == k.seg.t1) {  // (at the end: t1 = t0, and so on)
+                if (k.seg.t1 == k.seg.t0) return f;
+                walk_next<RT>(p, k);
+                publish();
+                at_t = k.seg.t0;
+            }
             f.tiles = min(k.seg.t1 - at_t, 32 / NP);
             if (f.tiles == 0) return f;
             const int pg = at_t * NP + lane;
             if (lane < f.tiles * NP && (long long)pg << p.w.lgP < k.s.len) {
                 const int x = kv8_unit(p.w, k.s, pg, k.seg.h);
-                if (x >= 0) f.have = 1, f.unit = x, f.ks = p.w.ks[x], f.vs = p.w.vs[x];
+                if (x >= 0) f.have = 1, f.unit = x;
             }
             at_t += f.tiles;
-            if (at_t == k.seg.t1) {
-                walk_next<RT>(p, k);
-                publish();
-                at_t = k.seg.t0;
-            }
             return f;
         };
         Batch nxt = fetch();
         bool ok = true;
         while (ok && nxt.tiles) {
             const Batch cur = nxt;
-            nxt.tiles = -1;
+            float ks = 0.0f, vs = 0.0f;  // of this lane's page
             for (int i = 0; ok && i < cur.tiles; ++i) {
                 const int at = i * NP, j = lane - at;
                 if (use > 0 && !(ok = warp_wait(&br.kempty[st], (use - 1) & 1, err, abort))) break;
@@ -505,14 +537,12 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_attend(const __grid_constan
                 }
                 __syncwarp();
                 if (mine) tma_page(&p.kmap, ksm + st * kStage + j * P * HDW, cur.unit, &br.kfull[st]);
-                // The next batch's entries are under way while this tile's wait.
-                if (nxt.tiles < 0) nxt = fetch();
-                Meta& m = z.meta[mt];
-                const unsigned valid = __ballot_sync(~0u, mine && cur.have) >> at;
-                if (mine) m.ks[j] = cur.ks, m.vs[j] = cur.vs;
-                if (lane == at) m.valid = (int)valid;
-                __syncwarp();
-                if (lane == at) mbar_arrive(&br.mfull[mt]);
+                if (i == 0) {
+                    // The batch's scales, and the next batch's entries, are on
+                    // their way while the first tile is.
+                    if (cur.have) ks = p.w.ks[cur.unit], vs = p.w.vs[cur.unit];
+                    nxt = fetch();
+                }
                 if (use > 0 && !(ok = warp_wait(&br.vempty[st], (use - 1) & 1, err, abort))) break;
                 if (lane == at) {
                     z.vfills[st] += 1;
@@ -520,6 +550,12 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_attend(const __grid_constan
                 }
                 __syncwarp();
                 if (mine) tma_page(&p.vmap, vsm + st * kStage + j * P * HDW, cur.unit, &br.vfull[st]);
+                Meta& m = z.meta[mt];
+                const unsigned valid = __ballot_sync(~0u, mine && cur.have) >> at;
+                if (mine) m.ks[j] = ks, m.vs[j] = vs;
+                if (lane == at) m.valid = (int)valid;
+                __syncwarp();
+                if (lane == at) mbar_arrive(&br.mfull[mt]);
                 if (++st == S) st = 0, ++use;
                 if (++mt == kMeta) mt = 0;
             }
