@@ -82,19 +82,49 @@ __device__ __forceinline__ PageRows page_rows(const Kv8View& w, const Kv8Seq& s,
     return r;
 }
 
+// How the threads of a CTA walk the items of a page's rows, one by one: items of
+// a row, and what a step of all threads adds.
+struct RowWalk {
+    int per_row, drow, dcol;
+    uint32_t inv;  // ceil(2^16 / per_row): a thread's row without a division
+};
+
+RowWalk row_walk(int per_row, int threads)
+{
+    return {per_row, threads / per_row, threads % per_row, (65535u + per_row) / per_row};
+}
+
+// Row `row` (at p) and item `col` of it that the thread is at.
+template <typename T>
+struct RowAt {
+    T* p;
+    int col;
+    __device__ __forceinline__ RowAt(const RowWalk& w, T* base, long long ld)
+    {
+        const int row = (int)(threadIdx.x * w.inv >> 16);
+        col = (int)threadIdx.x - row * w.per_row;
+        p = base + row * ld;
+    }
+    __device__ __forceinline__ void step(const RowWalk& w, long long ld, long long dld)
+    {
+        p += dld;
+        col += w.dcol;
+        if (col >= w.per_row) col -= w.per_row, p += ld;
+    }
+};
+
 struct AppendArgs {
     Kv8View w;
     const void* src[2];  // k, v
     long long ld[2];
     int vec[2];
-    int span;  // pages that max_rows rows can touch
+    RowWalk walk;
 };
 
 // One CTA per (sequence, page of it that rows fall into, head, k or v): a
 // thread holds its vectors of the new rows from the maximum to the codes, so
 // the rows are read once, and a chain of three dependent loads (length, page,
-// old scale) is all that a single token waits for.  Memory-bound: 2048 prompt
-// tokens of 8 sequences (bf16, 4 heads of 128, 50 MB) 12 us.
+// old scale) is all that a single token waits for.
 template <typename T>
 __global__ void __launch_bounds__(kAppendMax) k_kv8_append(const AppendArgs a)
 {
@@ -102,22 +132,22 @@ __global__ void __launch_bounds__(kAppendMax) k_kv8_append(const AppendArgs a)
     __shared__ uint32_t red[kAppendMax / 32];
     pdl_wait();
     const Kv8View& w = a.w;
-    const int h = blockIdx.y, kv = blockIdx.z, b = blockIdx.x / a.span, threads = blockDim.x;
-    const Kv8Seq s = kv8_seq(w, b);
-    const PageRows r = page_rows(w, s, blockIdx.x % a.span);
+    const int h = blockIdx.y >> 1, kv = blockIdx.y & 1, threads = blockDim.x;
+    const Kv8Seq s = kv8_seq(w, blockIdx.z);
+    const PageRows r = page_rows(w, s, blockIdx.x);
     if (r.hi <= r.lo) return;
     const T* src = static_cast<const T*>(a.src[kv]) + r.row * a.ld[kv] + (long long)h * w.hd;
-    // Vector q of the rows: row q / per_row, element (q % per_row) * VE.
-    const int per_row = w.hd / VE, n = (r.hi - r.lo) * per_row, had = r.lo - (r.at << w.lgP);
+    // The rows' vectors, in order.
+    const int n = (r.hi - r.lo) * a.walk.per_row, had = r.lo - (r.at << w.lgP);
     uint4 x[kVecs];
-    const int row0 = threadIdx.x / per_row, col0 = threadIdx.x % per_row, drow = threads / per_row, dcol = threads % per_row;
     {
-        int row = row0, col = col0;
+        RowAt<const T> at(a.walk, src, a.ld[kv]);
+        const long long dld = a.walk.drow * a.ld[kv];
 #pragma unroll
         for (int i = 0; i < kVecs; ++i) {
             x[i] = make_uint4(0, 0, 0, 0);
             if ((int)threadIdx.x + i * threads < n) {
-                const T* p = src + row * a.ld[kv] + col * VE;
+                const T* p = at.p + at.col * VE;
                 if (a.vec[kv]) {
                     x[i] = *reinterpret_cast<const uint4*>(p);
                 } else {
@@ -126,8 +156,7 @@ __global__ void __launch_bounds__(kAppendMax) k_kv8_append(const AppendArgs a)
                     for (int j = 0; j < VE; ++j) e[j] = p[j];
                 }
             }
-            row += drow, col += dcol;
-            if (col >= per_row) col -= per_row, ++row;
+            at.step(a.walk, a.ld[kv], dld);
         }
     }
     const int unit = kv8_unit(w, s, r.at, h);
@@ -190,58 +219,81 @@ __global__ void __launch_bounds__(kAppendMax) k_kv8_append(const AppendArgs a)
 // ------------------------------------------------------------------- read --
 
 constexpr int kReadThreads = 256;
-constexpr int kReadAtOnce = 8;  // groups of four codes that a thread loads before it stores
+constexpr int kReadAtOnce = 4;  // groups of eight codes that a thread loads before it stores
 
 struct ReadArgs {
     Kv8View w;
     void* dst[2];
     long long ld[2];
     int vec[2];
-    int span;
+    RowWalk walk;
 };
 
+// Eight consecutive elements, in one store where the address allows it.
+template <typename T>
+__device__ __forceinline__ void store8(T* p, bool vec, const float (&x)[8])
+{
+    if (!vec) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[i] = from_f<T>(x[i]);
+    } else if constexpr (sizeof(T) == 4) {
+        asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(x[0]), "f"(x[1]), "f"(x[2]),
+                     "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7])
+                     : "memory");
+    } else {
+        uint4 v;
+        T* t = reinterpret_cast<T*>(&v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] = from_f<T>(x[i]);
+        *reinterpret_cast<uint4*>(p) = v;
+    }
+}
+
 // One CTA per (sequence, page, head, k or v), like the append; a thread takes
-// four codes at a time.  CTA m = 0 of a sequence also zeroes its rows before
+// eight codes at a time.  CTA m = 0 of a sequence also zeroes its rows before
 // position 0.
 template <typename T>
 __global__ void __launch_bounds__(kReadThreads) k_kv8_read(const ReadArgs a)
 {
     pdl_wait();
     const Kv8View& w = a.w;
-    const int h = blockIdx.y, kv = blockIdx.z, b = blockIdx.x / a.span, m = blockIdx.x % a.span;
-    const Kv8Seq s = kv8_seq(w, b);
+    const int h = blockIdx.y >> 1, kv = blockIdx.y & 1, m = blockIdx.x;
+    const Kv8Seq s = kv8_seq(w, blockIdx.z);
     const PageRows r = page_rows(w, s, m);
-    const int q4 = w.hd >> 2;
+    const long long ld = a.ld[kv], dld = a.walk.drow * ld;
+    const bool vec = a.vec[kv];
     T* out = static_cast<T*>(a.dst[kv]) + (long long)h * w.hd;
-    const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (m == 0)
-        for (int g = threadIdx.x; g < min(s.n, max(s.n - s.len, 0)) * q4; g += kReadThreads)
-            store4<T>(out + (s.row0 + g / q4) * a.ld[kv] + g % q4 * 4, a.vec[kv], zero);
+    if (m == 0 && s.n > s.len) {
+        const float zero[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        RowAt<T> at(a.walk, out + s.row0 * ld, ld);
+        for (int g = threadIdx.x; g < min(s.n, s.n - s.len) * a.walk.per_row; g += kReadThreads) {
+            store8<T>(at.p + at.col * 8, vec, zero);
+            at.step(a.walk, ld, dld);
+        }
+    }
     if (r.hi <= r.lo) return;
     const int unit = kv8_unit(w, s, r.at, h);
     const float sc = unit >= 0 ? (kv ? w.vs : w.ks)[unit] : 0.0f;
-    const int8_t* page = (kv ? w.v : w.k) + ((size_t)max(unit, 0) * w.P + (r.lo & (w.P - 1))) * w.hd;
-    const int n = (r.hi - r.lo) * q4;
-    const int drow = kReadThreads / q4, dcol = kReadThreads % q4;
-    int row = threadIdx.x / q4, col = threadIdx.x % q4;
+    const uint2* page = reinterpret_cast<const uint2*>((kv ? w.v : w.k) + ((size_t)max(unit, 0) * w.P + (r.lo & (w.P - 1))) * w.hd);
+    const int n = (r.hi - r.lo) * a.walk.per_row;
+    RowAt<T> at(a.walk, out + r.row * ld, ld);
     for (int g0 = threadIdx.x; g0 < n; g0 += kReadAtOnce * kReadThreads) {
-        uint32_t c[kReadAtOnce];
+        uint2 c[kReadAtOnce];
 #pragma unroll
         for (int i = 0; i < kReadAtOnce; ++i) {
             const int g = g0 + i * kReadThreads;
-            c[i] = unit >= 0 && g < n ? reinterpret_cast<const uint32_t*>(page)[g] : 0u;
+            c[i] = unit >= 0 && g < n ? page[g] : make_uint2(0u, 0u);
         }
 #pragma unroll
         for (int i = 0; i < kReadAtOnce; ++i) {
             // The bytes, offset by 128, as the low bits of 2^23.
-            const uint32_t u = c[i] ^ 0x80808080u;
-            float x[4];
+            const uint32_t u[2] = {c[i].x ^ 0x80808080u, c[i].y ^ 0x80808080u};
+            float x[8];
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                x[k] = (__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + k)) - 8388736.0f) * sc;
-            if (g0 + i * kReadThreads < n) store4<T>(out + (r.row + row) * a.ld[kv] + col * 4, a.vec[kv], x);
-            row += drow, col += dcol;
-            if (col >= q4) col -= q4, ++row;
+            for (int k = 0; k < 8; ++k)
+                x[k] = (__uint_as_float(__byte_perm(u[k >> 2], 0x4b000000u, 0x7440 + (k & 3))) - 8388736.0f) * sc;
+            if (g0 + i * kReadThreads < n) store8<T>(at.p + at.col * 8, vec, x);
+            at.step(a.walk, ld, dld);
         }
     }
 }
@@ -271,17 +323,17 @@ int quantr_kv8_append_dev(const void* k, long long ldk, const void* v, long long
     a.w = kv8_view(pool, tables, batch, layer);
     const int bytes = type == QUANTR_TYPE_F32 ? 4 : 2;
     a.src[0] = k, a.src[1] = v, a.ld[0] = ldk, a.ld[1] = ldv;
-    a.vec[0] = aligned16(k, ldk, bytes), a.vec[1] = aligned16(v, ldv, bytes);
-    a.span = span_of(pool, batch->max_rows);
-    if ((long long)a.span * batch->B > 0x7fffffffll || pool->n_kv_heads > 65535) return QUANTR_ERR_TOO_LARGE;
+    a.vec[0] = aligned(k, ldk, bytes, 16), a.vec[1] = aligned(v, ldv, bytes, 16);
+    if (batch->B > 65535 || pool->n_kv_heads > 32767) return QUANTR_ERR_TOO_LARGE;
     // Threads that hold the most rows a page can get, kVecs vectors each.
-    const int vecs = std::min(batch->max_rows, pool->page_tokens) * pool->head_dim * bytes / 16;
+    const int per_row = pool->head_dim * bytes / 16, vecs = std::min(batch->max_rows, pool->page_tokens) * per_row;
     const int threads = (std::max(vecs / kVecs, std::min(vecs, 64)) + 31) / 32 * 32;
+    a.walk = row_walk(per_row, threads);
     LaunchCfg c;
     c.stream = (cudaStream_t)stream;
     return kv8_done(with_type(type, [&](auto* t) {
         using T = std::remove_const_t<std::remove_pointer_t<decltype(t)>>;
-        return launch_ex(k_kv8_append<T>, dim3(a.span * batch->B, pool->n_kv_heads, 2), threads, 0, c, a);
+        return launch_ex(k_kv8_append<T>, dim3(span_of(pool, batch->max_rows), 2 * pool->n_kv_heads, batch->B), threads, 0, c, a);
     }));
 }
 
@@ -296,14 +348,14 @@ int quantr_kv8_read_dev(void* k, long long ldk, void* v, long long ldv, uint32_t
     a.w = kv8_view(pool, tables, batch, layer);
     const int bytes = type == QUANTR_TYPE_F32 ? 4 : 2;
     a.dst[0] = k, a.dst[1] = v, a.ld[0] = ldk, a.ld[1] = ldv;
-    a.vec[0] = aligned4(k, ldk, bytes), a.vec[1] = aligned4(v, ldv, bytes);
-    a.span = span_of(pool, batch->max_rows);
-    if ((long long)a.span * batch->B > 0x7fffffffll || pool->n_kv_heads > 65535) return QUANTR_ERR_TOO_LARGE;
+    a.vec[0] = aligned(k, ldk, bytes, 8 * bytes), a.vec[1] = aligned(v, ldv, bytes, 8 * bytes);
+    if (batch->B > 65535 || pool->n_kv_heads > 32767) return QUANTR_ERR_TOO_LARGE;
+    a.walk = row_walk(pool->head_dim / 8, kReadThreads);
     LaunchCfg c;
     c.stream = (cudaStream_t)stream;
     return kv8_done(with_type(type, [&](auto* t) {
         using T = std::remove_const_t<std::remove_pointer_t<decltype(t)>>;
-        return launch_ex(k_kv8_read<T>, dim3(a.span * batch->B, pool->n_kv_heads, 2), kReadThreads, 0, c, a);
+        return launch_ex(k_kv8_read<T>, dim3(span_of(pool, batch->max_rows), 2 * pool->n_kv_heads, batch->B), kReadThreads, 0, c, a);
     }));
 }
 

@@ -194,34 +194,8 @@ __device__ __forceinline__ void load4(const T* p, bool vec, float (&x)[4])
     }
 }
 
-template <typename T>
-__device__ __forceinline__ void store4(T* p, bool vec, const float (&x)[4])
-{
-    if (vec) {
-        if constexpr (sizeof(T) == 4) {
-            *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
-        } else {
-            uint2 a;
-            T* t = reinterpret_cast<T*>(&a);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) t[i] = from_f<T>(x[i]);
-            *reinterpret_cast<uint2*>(p) = a;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[i] = from_f<T>(x[i]);
-    }
-}
-
-// Whether rows of `ld` elements of `bytes` each allow aligned loads of four.
-inline bool aligned4(const void* p, long long ld, int bytes)
-{
-    return ((uintptr_t)p % (4 * bytes)) == 0 && ld % 4 == 0;
-}
-
-// Whether head slices of such rows (whole multiples of 16 elements) allow
-// 16-byte loads.
-inline bool aligned16(const void* p, long long ld, int bytes) { return ((uintptr_t)p & 15) == 0 && ld * bytes % 16 == 0; }
+// Whether rows of `ld` elements of `bytes` each begin at multiples of `to`.
+inline bool aligned(const void* p, long long ld, int bytes, int to) { return (uintptr_t)p % to == 0 && ld * bytes % to == 0; }
 
 // Calls f with a null T* of the element type.
 template <typename F>

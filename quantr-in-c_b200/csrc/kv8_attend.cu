@@ -1179,7 +1179,7 @@ int quantr_kv8_attend_dev(void* out, long long ldo, const void* q, long long ldq
     AttendParams p{};
     p.w = kv8_view(pool, tables, batch, layer);
     p.q = q, p.out = out, p.lse = lse, p.ldq = ldq, p.ldo = ldo;
-    p.vec = aligned4(q, ldq, type == QUANTR_TYPE_F32 ? 4 : 2);
+    p.vec = type == QUANTR_TYPE_F32 ? aligned(q, ldq, 4, 16) : aligned(q, ldq, 2, 8);
     p.H = n_heads, p.G = n_heads / pool->n_kv_heads, p.window = window;
     p.inv_g = p.G == 1 ? 0 : (unsigned)(((1ull << 32) + p.G - 1) / p.G);
     p.scale2 = (float)((double)scale * 1.4426950408889634);
