@@ -537,8 +537,9 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LpArgs a)
     } else if (slice) {
         return;
     }
-    // The row's sums, from every warp's (64 places, the others empty), in each
-    // warp: the alternatives need lse.
+    // The row's sums, from every warp's (64 places, the others empty), and its
+    // results: one warp's work, the others' issue slots are the next row's.
+    if (warp) return;
     WideSums sum = z.part[lane];
     if (a.split * kLpWarps > 32) {
         const WideSums u = z.part[32 + lane];
@@ -563,7 +564,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LpArgs a)
             a.logprob[row] = (float)lp;
         }
     }
-    for (int i = tid; i < a.k; i += kLpThreads) {
+    for (int i = lane; i < a.k; i += 32) {
         const u64 key = z.tops[i];
         if (a.top_id) a.top_id[(size_t)row * a.k + i] = key ? (int)~(uint32_t)key : -1;
         if (a.top_lp) a.top_lp[(size_t)row * a.k + i] = bad ? NAN : key ? (float)(lp_value(key) * a.inv_t - lse) : -INFINITY;
