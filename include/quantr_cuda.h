@@ -551,10 +551,11 @@ int quantr_kv8_read_dev(void* k, long long ldk, void* v, long long ldv, uint32_t
  * q and out have `type` (F32/F16/BF16).  A row that sees nothing (position
  * below 0, all of its pages missing) gives out = 0, lse = -inf; a page that is
  * missing counts as masked.  A query or a scale that is not finite gives NaN.
- * max_len is the longest sequence expected: it sizes the split of long
- * sequences over the GPU and the workspace; longer ones are right, only
- * slower.  The workspace must be 256-byte aligned and its first 4096 bytes zero
- * before its first use; every call leaves them zero, so it is zeroed once.
+ * max_len (>= 0) is the longest sequence expected; neither the split of long
+ * sequences over the GPU nor the workspace depends on it, since the lengths are
+ * read on the device.  The workspace must be 256-byte aligned and its first 4096
+ * bytes zero before its first use; every call leaves them zero, so it is zeroed
+ * once (and again after a call that ended with QUANTR_ERR_DEVICE_TIMEOUT).
  * Calls that may overlap need a workspace each. */
 size_t quantr_kv8_attend_workspace_bytes(const quantr_kv8_pool* pool, const quantr_kv8_batch* batch, int n_heads,
                                          int max_len);

@@ -21,14 +21,35 @@
 // the maximum of a long row lies, and a page has one scale, which the join
 // applies once per page instead of once per token.
 //
-// Work is a flat list of (sequence, KV head, row tile, 128-token tile); every
-// CTA takes an equal, contiguous share, so ragged batches and long sequences
-// fill the GPU alike.  A row tile that several CTAs share is joined by the one
-// that finishes last, in the order of the tokens (the result does not depend on
-// who that is).
+// Work is shared out in (sequence, KV head, row tile of up to 16 rows) x
+// 128-token tiles; see walk_begin.  A row tile that several CTAs share is joined
+// by the one that finishes last, in the order of the tokens (the result does not
+// depend on who that is).
 //
-// Roles (320 threads): warps 0-3 softmax (thread = token), 4-7 join (thread =
-// output element), 8 copies (TMA), 9 issues the MMAs.
+// Roles (320 threads, two CTAs per SM): warps 0-3 softmax (thread = token), 4-7
+// join (thread = output element), 8 copies (TMA, up to 6 stages ahead), 9 issues
+// the MMAs.  S has two TMEM buffers, so a tile's scores are computed while the
+// tile before is weighted, and its outputs while the next is scored.
+//
+// What bounds it, and what it measured (B200, 6.54 TB/s copy; launches back to
+// back in a graph, inputs in rotation):
+//   8 sequences of 200 to 262 thousand tokens, 32/4 heads of 128, bf16: 1.87 GB
+//     in 292 us, 6.4 TB/s: memory.  4 of 100 to 131 thousand (459 MB): 86.7 us,
+//     5.3 TB/s; the 16 us above the copy rate are launch, start (length, page
+//     entry and keys are loads that wait for one another) and the join of the
+//     18 to 20 CTAs that share a row tile.
+//   64 sequences of 640 to 1152 tokens, fp32 (61 MB): 20.0 us, 3.1 TB/s; the start
+//     and the longest CTA's tiles, one after the other.
+//   1 sequence of 513 tokens: 8.6 us; latency, of one tile and the join of five.
+//   6 prompt chunks of 64 tokens (2.2 GFLOP): 47.1 us; issue slots are 53 % used,
+//     the tensor pipe 4 %.  512 tokens after 3584 (32 GFLOP): 254 us; a tile takes
+//     4000 cycles (clock readings), nearly all in the softmax warps, of which two
+//     CTAs per SM keep two in flight.
+// Tried and not kept, each beside what it was at that step, in us: one reference
+// weight per warp's 32 tokens instead of per page (no exchange between warps, but
+// four outputs per tile to join: long contexts 94 -> 103); scoring a tile ahead
+// of the weights, which then wait for the next tile's keys (94 -> 108); row tiles
+// of 32, whose registers leave one CTA per SM (chunks of 64 fp32 rows 67 -> 83).
 #include "kv8.cuh"
 
 #include <algorithm>

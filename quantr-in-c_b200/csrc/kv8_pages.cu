@@ -50,8 +50,9 @@ struct SelectArgs {
 constexpr int kSelectCtas = 8, kSelectThreads = 1024;
 
 // One cluster: the references are zeroed, the cluster meets, and its warps take
-// the slots one by one, counting the pages they copy.  One launch: 4 us for 64
-// slots of 20 pages.  (Integer counts: their order does not matter.)
+// the slots one by one, counting the pages they copy (integers: their order does
+// not matter).  Latency-bound: 3.7 us for 64 slots of 10 to
+// 18 pages, 2.2 for 16 of 9.
 __global__ void __launch_bounds__(kSelectThreads) __cluster_dims__(kSelectCtas, 1, 1) k_kv8_select(const SelectArgs a)
 {
     pdl_wait();
@@ -107,7 +108,8 @@ constexpr int kChunk = kCopyThreads * kAtOnce;  // vectors that a CTA copies at 
 
 // Work item (copy, chunk of its page): 16 KB of codes, or the page's scales.
 // CTAs take the items in turn, so a few large pages fill the GPU as well as
-// many small ones.  Memory-bound: 1.7 GB moved (read and written) in 260 us.
+// many small ones.  Memory-bound: 250 pages of 3.1 MB, 1.57 GB read and written,
+// in 245 us, 6.4 TB/s.
 __global__ void __launch_bounds__(kCopyThreads) k_kv8_copy(const CopyArgs a)
 {
     pdl_wait();
@@ -166,7 +168,9 @@ struct PlanArgs {
     int* err;
 };
 
-// One CTA, thread i plans sequence i.
+// One CTA, thread i plans sequence i: what it needs, a prefix sum of that, the
+// free pages up to the total.  Latency-bound: with its copies (15 pages of 0.7
+// MB, 22 MB moved) an extend of 16 sequences takes 7.8 us.
 __global__ void __launch_bounds__(kPlanThreads) k_kv8_extend(const PlanArgs a)
 {
     __shared__ int red[33], tails[kPlanThreads];
@@ -273,7 +277,8 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv8_extend(const PlanArgs a)
 // ---------------------------------------------------------------- compact --
 
 // One CTA: n_live, then the i-th page in use at or past it to the i-th hole
-// before it.
+// before it: the fewest pages move, and none is read and written.  With the
+// copies, 1.69 GB read and written: 263 us, 6.4 TB/s.
 __global__ void __launch_bounds__(kPlanThreads) k_kv8_compact(const PlanArgs a)
 {
     __shared__ int red[33];
