@@ -20,7 +20,7 @@ LIB = os.path.join(LIBDIR, "libquantr_cuda.so")
 SOURCES = ["gemv.cu", "engine.cu", "tc.cu", "moe.cu", "api.cu", "noalloc.cu", "decode.cu", "decode_persist.cu",
            "kv8.cu", "kv8_attend.cu", "kv8_pages.cu", "logprobs.cu"]
 HEADERS = ["formats.cuh", "kernels.cuh", "device_common.cuh", "quant_decode.cuh", "launch_util.cuh",
-           "libm_ref.cuh", "engine_act.cuh", "decode_persist.cuh", "kv8.cuh"]
+           "libm_ref.cuh", "engine_act.cuh", "decode_persist.cuh", "kv8.cuh", "kv8_join.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -51,6 +51,7 @@
 // of the weights, which then wait for the next tile's keys (94 -> 108); row tiles
 // of 32, whose registers leave one CTA per SM (chunks of 64 fp32 rows 67 -> 83).
 #include "kv8.cuh"
+#include "kv8_join.cuh"
 
 #include <algorithm>
 #include <cmath>
@@ -64,9 +65,6 @@ constexpr int kThreads = 320;
 constexpr int kTile = 128;     // tokens per tile
 constexpr int kMeta = 16;      // rings of the segments, and of the tiles' page scales
 constexpr int kMaxStages = 6;
-constexpr int kChunk = 32;     // parts of a row tile joined at once
-constexpr int kGroup = 16;     // more of them than kChunk are joined in groups first
-constexpr int kMaxCtas = 512;
 constexpr int kSlack = 5;      // tiles that sharing out by row tiles may cost the longest CTA
 
 struct AttendParams {
@@ -81,7 +79,7 @@ struct AttendParams {
     float scale2;  // scale * log2(e)
     int vec;       // query rows allow aligned loads of four
     int stages, nS, nO, tmem_cols;
-    int* counters;  // [2][kMaxCtas] by a row tile's (a group's) first CTA, zero between calls
+    int* counters;  // see kv8_join.cuh; zero between calls
     float* part;    // 2 per CTA: o [RT][128], m [RT], l [RT]
 };
 
@@ -1031,22 +1029,16 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_attend(const __grid_constan
         for (int i = 0; ok && i < n_shared; ++i) {
             const Seg q = i ? shared1 : shared0;
             bool last = false;
-            int n = q.c1 - q.c0 + 1;
-            const int g0 = q.c0 + (me - q.c0) / kGroup * kGroup;
-            const bool grouped = n > kChunk;
-            int* counter = p.counters + (grouped ? g0 : kMaxCtas + q.c0);
-            const float* base = p.part + 2 * (size_t)(grouped ? g0 : q.c0) * kPart;
-            size_t stride = 2 * kPart;
-            int gn = grouped ? min(kGroup, q.c1 - g0 + 1) : n;
+            const int g0 = join_group(q.c0, me);
+            const bool grouped = join_grouped(q.c0, q.c1);
 #pragma unroll 1
-            for (int level = grouped ? 0 : 1; level < 2; ++level) {
-                if (!(ok = last_of(counter, gn, last)) || !last) break;
-                const bool shift = level || g0 == q.c0;
-                join_parts(base, gn, stride, shift, level ? nullptr : const_cast<float*>(base) + (shift ? kPart : 0), q);
-                counter = p.counters + kMaxCtas + q.c0;
-                base = p.part + 2 * (size_t)q.c0 * kPart;
-                stride = 2 * kPart * kGroup;
-                gn = (n + kGroup - 1) / kGroup;
+            for (int step = join_first(q.c0, q.c1, me); step < 2; ++step) {
+                const JoinStep s = join_step(step, q.c0, q.c1, me);
+                if (!(ok = last_of(p.counters + s.counter, s.n, last)) || !last) break;
+                const bool shift = step || g0 == q.c0;
+                const float* base = p.part + 2 * (size_t)(step ? q.c0 : g0) * kPart;
+                const size_t stride = 2 * kPart * (step && grouped ? kJoinGroup : 1);
+                join_parts(base, s.n, stride, shift, step ? nullptr : const_cast<float*>(base) + (shift ? kPart : 0), q);
             }
         }
     }
@@ -1110,7 +1102,7 @@ Plan make_plan(int lgP)
     const size_t room = (r.occ == 2 ? 113 : 226) * 1024;
     r.stages = (int)std::min<size_t>(kMaxStages, (room - fixed) / (2 * kTile * HDW));
     r.smem = fixed + (size_t)r.stages * 2 * kTile * HDW;
-    r.grid = r.occ * device_sm_count();
+    r.grid = std::min(r.occ * device_sm_count(), kJoinCtas);
     return r;
 }
 

@@ -1,0 +1,45 @@
+"""GPU: attention over the 8-bit cache where long sequences lie among short ones,
+so that neighbouring row tiles are each shared by more than 32 CTAs, call after
+call on one workspace.  Formulas and tolerances are test_kv8_gpu.py's.
+"""
+import pytest
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+from test_kv8_gpu import BF16, F32, Cache, attend, check, query, want_attend  # noqa: E402
+
+SHAPES = [
+    # KV, G, lens: on 296 CTAs the last group of one row tile is one CTA, which
+    # is also the first of the next row tile
+    (4, 1, [65600, 1000]),
+    (4, 1, [131072, 64000]),
+    (4, 8, [100000] + [2000] * 21),
+    (4, 8, [131072] + [2000] * 29),
+    (8, 2, [100000] + [2000] * 5),
+    # and others around them
+    (2, 4, [70000, 1, 129, 0, 3000]),
+    (1, 1, [40000, 150000]),
+]
+
+
+@pytest.mark.parametrize("type_", [F32, BF16])
+def test_uneven_long_contexts_on_one_workspace(qr_gpu, type_):
+    """Every output is written and right, the counters are zero after every call
+    (attend() looks), and the bits stay the same from call to call."""
+    ws = torch.zeros(1 << 23, dtype=torch.uint8, device="cuda")
+    made = []
+    for i, (KV, G, lens) in enumerate(SHAPES):
+        c = Cache(qr_gpu, lens, KV, 64, 64, seed=40 + i)
+        q = query(len(lens), KV * G, 64, type_, seed=50 + i)
+        made.append((c, q, [1] * len(lens)))
+    first = []
+    for c, q, rows in made:
+        got = attend(qr_gpu, c, q, rows, ws=ws)
+        check(c, q, got, want_attend(c, q, rows))
+        first.append(got)
+    for _ in range(20):
+        for (c, q, rows), want in zip(made, first):
+            got = attend(qr_gpu, c, q, rows, ws=ws)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert qr_gpu.device_status() == 0
