@@ -330,7 +330,7 @@ int quantr_kv8_append_dev(const void* k, long long ldk, const void* v, long long
     if (batch->B > 65535 || pool->n_kv_heads > 32767) return QUANTR_ERR_TOO_LARGE;
     // Threads that hold the most rows a page can get, kVecs vectors each.
     const int per_row = pool->head_dim * bytes / 16, vecs = std::min(batch->max_rows, pool->page_tokens) * per_row;
-    const int threads = (std::max(vecs / kVecs, std::min(vecs, 64)) + 31) / 32 * 32;
+    const int threads = (std::max((vecs + kVecs - 1) / kVecs, std::min(vecs, 64)) + 31) / 32 * 32;
     a.walk = row_walk(per_row, threads);
     LaunchCfg c;
     c.stream = (cudaStream_t)stream;
