@@ -478,7 +478,8 @@ int quantr_gemv_noalloc_dev(float* out, long long ldo, const float* x, long long
  * src/runtime.c:74-92) and whose samplers see one token's logits.
  *
  * All pointers inside the structs and arguments are device pointers, except the
- * structs themselves, which the host reads during the call.  Every call is
+ * structs themselves, which the host reads during the call.  Pointers are
+ * multiples of their elements' size (QUANTR_ERR_BAD_ARG if not).  Every call is
  * asynchronous on `stream`, allocates nothing and can be captured (the first
  * call on a device allocates its error word: make it before any capture).
  * What only the device can see - a slot or page id out of range, a table too

@@ -321,7 +321,7 @@ int quantr_kv8_append_dev(const void* k, long long ldk, const void* v, long long
     int rc = kv8_check_call(pool, tables, batch, layer, type);
     if (rc || batch->B == 0 || batch->max_rows == 0) return rc;
     const long long need = (long long)pool->n_kv_heads * pool->head_dim;
-    if ((rc = kv8_check_rows(k, ldk, need)) || (rc = kv8_check_rows(v, ldv, need))) return rc;
+    if ((rc = kv8_check_rows(k, ldk, need, type)) || (rc = kv8_check_rows(v, ldv, need, type))) return rc;
     AppendArgs a{};
     a.w = kv8_view(pool, tables, batch, layer);
     const int bytes = type == QUANTR_TYPE_F32 ? 4 : 2;
@@ -346,7 +346,7 @@ int quantr_kv8_read_dev(void* k, long long ldk, void* v, long long ldv, uint32_t
     int rc = kv8_check_call(pool, tables, batch, layer, type);
     if (rc || batch->B == 0 || batch->max_rows == 0) return rc;
     const long long need = (long long)pool->n_kv_heads * pool->head_dim;
-    if ((rc = kv8_check_rows(k, ldk, need)) || (rc = kv8_check_rows(v, ldv, need))) return rc;
+    if ((rc = kv8_check_rows(k, ldk, need, type)) || (rc = kv8_check_rows(v, ldv, need, type))) return rc;
     ReadArgs a{};
     a.w = kv8_view(pool, tables, batch, layer);
     const int bytes = type == QUANTR_TYPE_F32 ? 4 : 2;

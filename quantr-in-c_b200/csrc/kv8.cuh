@@ -5,6 +5,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <initializer_list>
 
 #include "device_common.cuh"
 #include "kernels.cuh"
@@ -16,11 +17,19 @@ constexpr uint32_t T_F16 = QUANTR_TYPE_F16, T_BF16 = QUANTR_TYPE_BF16;
 
 inline bool kv8_float_type(uint32_t t) { return t == QUANTR_TYPE_F32 || t == T_F16 || t == T_BF16; }
 
+// Whether all addresses (null ones too) are multiples of an element's size: an
+// access at any other is a fault on the device.
+inline bool kv8_aligned(std::initializer_list<const void*> ps, size_t bytes = 4)
+{
+    for (const void* p : ps)
+        if ((uintptr_t)p % bytes) return false;
+    return true;
+}
+
 inline int kv8_check_pool(const quantr_kv8_pool* p)
 {
     if (!p || !p->k || !p->v || !p->k_scale || !p->v_scale) return QUANTR_ERR_BAD_ARG;
-    if (((uintptr_t)p->k | (uintptr_t)p->v) & 15) return QUANTR_ERR_BAD_ARG;
-    if (((uintptr_t)p->k_scale | (uintptr_t)p->v_scale) & 3) return QUANTR_ERR_BAD_ARG;
+    if (!kv8_aligned({p->k, p->v}, 16) || !kv8_aligned({p->k_scale, p->v_scale})) return QUANTR_ERR_BAD_ARG;
     if (p->n_pages <= 0 || p->n_layers <= 0 || p->n_kv_heads <= 0) return QUANTR_ERR_BAD_ARG;
     if (p->page_tokens != 32 && p->page_tokens != 64 && p->page_tokens != 128) return QUANTR_ERR_BAD_ARG;
     if (p->head_dim <= 0 || p->head_dim % 16) return QUANTR_ERR_BAD_ARG;
@@ -32,18 +41,20 @@ inline int kv8_check_pool(const quantr_kv8_pool* p)
 inline int kv8_check_tables(const quantr_kv8_tables* t)
 {
     if (!t || !t->table || !t->lens || !t->refs || t->slots <= 0 || t->max_pages <= 0) return QUANTR_ERR_BAD_ARG;
-    return QUANTR_OK;
+    return kv8_aligned({t->table, t->lens, t->refs}) ? QUANTR_OK : QUANTR_ERR_BAD_ARG;
 }
 
 // A batch of no sequences or no rows is allowed (the calls do nothing).
 inline int kv8_check_batch(const quantr_kv8_batch* b)
 {
-    return b && b->B >= 0 && b->max_rows >= 0 ? QUANTR_OK : QUANTR_ERR_BAD_ARG;
+    return b && b->B >= 0 && b->max_rows >= 0 && kv8_aligned({b->slot, b->start}) ? QUANTR_OK : QUANTR_ERR_BAD_ARG;
 }
 
-inline int kv8_check_rows(const void* p, long long ld, long long need)
+inline size_t kv8_type_bytes(uint32_t type) { return type == QUANTR_TYPE_F32 ? 4 : 2; }
+
+inline int kv8_check_rows(const void* p, long long ld, long long need, uint32_t type)
 {
-    return p && ld >= need ? QUANTR_OK : QUANTR_ERR_BAD_ARG;
+    return p && ld >= need && kv8_aligned({p}, kv8_type_bytes(type)) ? QUANTR_OK : QUANTR_ERR_BAD_ARG;
 }
 
 inline int kv8_check_call(const quantr_kv8_pool* pool, const quantr_kv8_tables* tables, const quantr_kv8_batch* batch, int layer,

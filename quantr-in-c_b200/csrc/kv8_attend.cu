@@ -1178,7 +1178,8 @@ int quantr_kv8_attend_dev(void* out, long long ldo, const void* q, long long ldq
         return QUANTR_ERR_BAD_ARG;
     if (batch->B == 0 || batch->max_rows == 0) return QUANTR_OK;
     const long long need = (long long)n_heads * pool->head_dim;
-    if ((rc = kv8_check_rows(out, ldo, need)) || (rc = kv8_check_rows(q, ldq, need))) return rc;
+    if ((rc = kv8_check_rows(out, ldo, need, type)) || (rc = kv8_check_rows(q, ldq, need, type))) return rc;
+    if (!kv8_aligned({lse})) return QUANTR_ERR_BAD_ARG;
     if (!workspace || ((uintptr_t)workspace & 255) ||
         workspace_bytes < quantr_kv8_attend_workspace_bytes(pool, batch, n_heads, max_len))
         return QUANTR_ERR_WORKSPACE;

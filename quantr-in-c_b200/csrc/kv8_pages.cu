@@ -370,7 +370,7 @@ int quantr_kv8_select_dev(const quantr_kv8_tables* to, const quantr_kv8_tables* 
     if (!rc) rc = kv8_check_tables(in);
     if (rc) return rc;
     if (!from || to->slots != in->slots || to->max_pages != in->max_pages || to->table == in->table ||
-        to->lens == in->lens || to->refs == in->refs)
+        to->lens == in->lens || to->refs == in->refs || !kv8_aligned({from}))
         return QUANTR_ERR_BAD_ARG;
     SelectArgs a{*to, *in, from, pool->n_pages, lg_tokens(pool), device_error_word()};
     LaunchCfg c;
@@ -410,7 +410,7 @@ int quantr_kv8_extend_dev(const quantr_kv8_pool* pool, const quantr_kv8_tables* 
                           const int* n_new, int B, int* grown, void* workspace, size_t workspace_bytes, void* stream)
 {
     int rc = pages_check(pool, tables, workspace, workspace_bytes);
-    if (!rc && (B < 0 || (!slot && B > tables->slots))) rc = QUANTR_ERR_BAD_ARG;
+    if (!rc && (B < 0 || (!slot && B > tables->slots) || !kv8_aligned({slot, n_new, grown}))) rc = QUANTR_ERR_BAD_ARG;
     if (!rc && B > kPlanThreads) rc = QUANTR_ERR_TOO_LARGE;
     if (rc || B == 0) return rc;
     PlanArgs a = plan_args(pool, tables, workspace);
@@ -427,6 +427,7 @@ int quantr_kv8_compact_dev(const quantr_kv8_pool* pool, const quantr_kv8_tables*
                            void* workspace, size_t workspace_bytes, void* stream)
 {
     int rc = pages_check(pool, tables, workspace, workspace_bytes);
+    if (!rc && !kv8_aligned({map, n_live})) rc = QUANTR_ERR_BAD_ARG;
     if (rc) return rc;
     PlanArgs a = plan_args(pool, tables, workspace);
     a.map = map, a.n_live = n_live;
@@ -441,7 +442,7 @@ int quantr_kv8_compact_dev(const quantr_kv8_pool* pool, const quantr_kv8_tables*
 int quantr_kv8_copy_pages_dev(const quantr_kv8_pool* pool, const int* dst, const int* src, int n, void* stream)
 {
     int rc = kv8_check_pool(pool);
-    if (!rc && (n < 0 || (n > 0 && (!dst || !src)))) rc = QUANTR_ERR_BAD_ARG;
+    if (!rc && (n < 0 || (n > 0 && (!dst || !src)) || !kv8_aligned({dst, src}))) rc = QUANTR_ERR_BAD_ARG;
     if (rc || n == 0) return rc;
     CopyArgs k{*pool, nullptr, n, src, dst, device_error_word(), nullptr, nullptr, 0};
     LaunchCfg c;

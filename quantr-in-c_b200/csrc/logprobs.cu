@@ -612,7 +612,8 @@ int quantr_logprobs_dev(const void* x, long long ldl, uint32_t type, int rows, i
         return QUANTR_ERR_BAD_ARG;
     if (k > kMaxTop) return QUANTR_ERR_TOO_LARGE;
     if (rows == 0) return QUANTR_OK;
-    if (!x || (uintptr_t)x % (type == QUANTR_TYPE_F32 ? 4 : 2) || (logprob && !token)) return QUANTR_ERR_BAD_ARG;
+    if (!x || !kv8_aligned({x}, kv8_type_bytes(type)) || (logprob && !token)) return QUANTR_ERR_BAD_ARG;
+    if (!kv8_aligned({token, logprob, entropy, lse, top_id, top_logprob})) return QUANTR_ERR_BAD_ARG;
     (void)workspace, (void)workspace_bytes;
     LpArgs a{};
     a.x = x, a.ldl = ldl, a.rows = rows, a.V = vocab, a.k = k, a.split = lp_split(rows, vocab);
