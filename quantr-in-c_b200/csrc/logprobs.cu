@@ -95,8 +95,9 @@ __device__ __forceinline__ float warp_max(float x)
     return y;
 }
 
+// A thread's sums are about 2^(c m - lo): see `take`.
 struct Sums {
-    float m, s, e;
+    float m, s, e, lo;
 };
 
 // Sums of more than one thread are held in 64 bits: a row's rounding is then
@@ -106,13 +107,13 @@ struct WideSums {
     double s, e;
 };
 
-// The warp's sums about their largest maximum; in all lanes.
-__device__ __forceinline__ WideSums join_warp(WideSums a, float c)
+// The warp's sums about their largest maximum; in all lanes.  `lo`: see Sums.
+__device__ __forceinline__ WideSums join_warp(WideSums a, float c, float lo = 0.0f)
 {
     const float m = warp_max(a.m);
     if (m > -INFINITY) {
         // (2^-200 is 0, and bounded it makes no 0 * -inf; NaN stays.)
-        const float d = lp_max_nan((a.m - m) * c, -200.0f), f = lp_ex2(d);
+        const float d = lp_max_nan((a.m - m) * c - lo, -200.0f), f = lp_ex2(d);
         a.e = (a.e + a.s * d) * f;
         a.s *= f;
     }
@@ -343,21 +344,27 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LpArgs a)
     const uint32_t ninf = sizeof(T) == 4 ? 0xff800000u : std::is_same_v<T, __half> ? 0xfc00fc00u : 0xff80ff80u;
     const uint4 none = make_uint4(ninf, ninf, ninf, ninf);
 
-    Sums st{-INFINITY, 0.0f, 0.0f};
+    Sums st{-INFINITY, 0.0f, 0.0f, 0.0f};
     // Tiles of a group: as few as keep the groups within kGroups.
     const int gt = (tiles + kGroups - 1) / kGroups;
     float gmax = -INFINITY;
     int left = gt, group = 0;
     const F2 c2 = f2(a.c, a.c);
+    // Whether a tile's exponents may be c x - (c m rounded), one instruction each:
+    // its rounding, `lo`, is then half a unit at most, and no logit is below the
+    // bound.
+    bool plain = false;
     // The running maximum takes `mt` in; the group's, too.
     auto raise = [&](float mt) {
         if (mt > st.m) {
+            plain = fabsf(mt * a.c) <= 8388608.0f && (mt - Low<T>::bound) * a.c > 200.0f;
+            const float lo = plain ? fmaf(mt, a.c, -(mt * a.c)) : 0.0f;
             if (st.m > -INFINITY) {
-                const float d = lp_max_nan((st.m - mt) * a.c, -200.0f), r = lp_ex2(d);
+                const float d = lp_max_nan((st.m - mt) * a.c + (lo - st.lo), -200.0f), r = lp_ex2(d);
                 st.e = fmaf(st.s, d, st.e) * r;
                 st.s *= r;
             }
-            st.m = mt;
+            st.m = mt, st.lo = lo;
         }
         gmax = fmaxf(gmax, mt);
         if (--left == 0) {
@@ -368,7 +375,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LpArgs a)
     auto one = [&](float y) {
         const float base = st.m == -INFINITY ? 0.0f : st.m;
         // 2^-200 is 0; the bound keeps -inf out of 0 * -inf and NaN in.
-        const float d = lp_max_nan((y - base) * a.c, -200.0f), p = lp_ex2(d);
+        const float d = lp_max_nan((y - base) * a.c + st.lo, -200.0f), p = lp_ex2(d);
         st.s += p;
         st.e = fmaf(p, d, st.e);
     };
@@ -377,7 +384,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LpArgs a)
 #pragma unroll
         for (int i = 1; i < kVecs; ++i) mt = fmaxf(mt, vec_max<T>(cur[i]));
         raise(mt);
-        if (fabsf(st.m * a.c) <= 3.402823466e38f && (st.m - Low<T>::bound) * a.c > 200.0f) {
+        if (plain) {
             const float ref = -st.m * a.c;
             const F2 r2 = f2(ref, ref);
             F2 s2 = f2(0.0f, 0.0f), e2 = s2;
@@ -401,8 +408,9 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LpArgs a)
             f2_get(e2, x0, x1);
             st.e += x0 + x1;
         } else {
-            // Nothing above the bound yet, or a maximum that c times has no
-            // float: a row of nothing but the type's lowest value, say.
+            // Nothing above the bound yet, or a maximum millions of temperatures
+            // from 0 (a row of nothing but the type's lowest value, say), whose
+            // product with c says nothing about differences: those come first.
 #pragma unroll 1
             for (int v = 0; v < kVecs; ++v) {
                 float f[VE];
@@ -460,7 +468,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LpArgs a)
         if (lane == __ffs(who) - 1) y = -INFINITY;
         if (lane == i) head_val = top;
     }
-    const WideSums mine = join_warp({st.m, st.s, st.e}, a.c);
+    const WideSums mine = join_warp({st.m, st.s, st.e}, a.c, st.lo);
     cluster_wait();
     if (warp < nw && lane < per_warp)
         for (int r = 0; r < a.split; ++r)
