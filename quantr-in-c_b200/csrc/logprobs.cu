@@ -51,6 +51,10 @@ struct LpArgs {
     int rows, V, k, split;
     double inv_t;  // 1 / temperature
     float c;       // times log2(e)
+    // Maxima m (above < m, |m| <= most) for which a tile's exponents are
+    // c x - (c m rounded), one instruction each: that rounding is then half a unit
+    // at most, and Low<T>::bound weighs nothing beside m.
+    float above, most;
     const int* token;
     float* logprob;
     float* entropy;
@@ -350,14 +354,11 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LpArgs a)
     float gmax = -INFINITY;
     int left = gt, group = 0;
     const F2 c2 = f2(a.c, a.c);
-    // Whether a tile's exponents may be c x - (c m rounded), one instruction each:
-    // its rounding, `lo`, is then half a unit at most, and no logit is below the
-    // bound.
-    bool plain = false;
+    bool plain = false;  // see LpArgs
     // The running maximum takes `mt` in; the group's, too.
     auto raise = [&](float mt) {
         if (mt > st.m) {
-            plain = fabsf(mt * a.c) <= 8388608.0f && (mt - Low<T>::bound) * a.c > 200.0f;
+            plain = mt > a.above && fabsf(mt) <= a.most;
             const float lo = plain ? fmaf(mt, a.c, -(mt * a.c)) : 0.0f;
             if (st.m > -INFINITY) {
                 const float d = lp_max_nan((st.m - mt) * a.c + (lo - st.lo), -200.0f), r = lp_ex2(d);
@@ -633,6 +634,9 @@ int quantr_logprobs_dev(const void* x, long long ldl, uint32_t type, int rows, i
     c.stream = (cudaStream_t)stream;
     return kv8_done(with_type(type, [&](auto* t) {
         using T = std::remove_const_t<std::remove_pointer_t<decltype(t)>>;
+        a.above = Low<T>::bound + 200.0f / a.c;
+        // (None where c times the bound has no float, which would be 0 * -inf.)
+        a.most = std::isfinite(Low<T>::bound * a.c) ? 8388608.0f / a.c : -1.0f;
         // Tiles of the longest slice, with one for the ragged ends.
         const int vecs = vocab / Vec<T>::n, per = (vecs + a.split - 1) / a.split;
         const int tiles = (per + kVecs * kLpThreads - 1) / (kVecs * kLpThreads) + 1;
