@@ -597,7 +597,8 @@ int quantr_kv8_compact_dev(const quantr_kv8_pool* pool, const quantr_kv8_tables*
 int quantr_kv8_copy_pages_dev(const quantr_kv8_pool* pool, const int* dst, const int* src, int n, void* stream);
 
 /* Log probabilities of rows of logits (x[r*ldl + v], v < vocab, type
- * F32/F16/BF16), y = x / temperature:
+ * F32/F16/BF16), y = x / temperature (finite, and at least 4.25e-39, so that
+ * log2(e) / temperature has a float):
  *   lse[r]     = ln sum_v exp(y_v)
  *   logprob[r] = y[token[r]] - lse[r]; 0 where token[r] is -1 (no token
  *                given), NaN where it is any other id outside the vocabulary

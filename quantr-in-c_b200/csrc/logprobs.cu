@@ -617,7 +617,7 @@ int quantr_logprobs_dev(const void* x, long long ldl, uint32_t type, int rows, i
 {
     if (!kv8_float_type(type)) return QUANTR_ERR_UNSUPPORTED_TYPE;
     if (rows < 0 || vocab <= 0 || k < 0 || ldl < vocab || !(temperature > 0.0f) || !std::isfinite(temperature) ||
-        !std::isfinite(1.0f / temperature))
+        !std::isfinite((float)(1.4426950408889634 / (double)temperature)))
         return QUANTR_ERR_BAD_ARG;
     if (k > kMaxTop) return QUANTR_ERR_TOO_LARGE;
     if (rows == 0) return QUANTR_OK;
