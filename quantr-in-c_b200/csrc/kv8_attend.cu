@@ -195,8 +195,8 @@ __device__ __forceinline__ int seq_tiles(const AttendParams& p, const Kv8Seq& s,
 {
     nrt = (s.n * p.G + RT - 1) / RT;
     const int have = (int)min((long long)max(s.len, 0), (long long)p.w.max_pages << p.w.lgP);
-    const int low = s.len - s.n - p.window + 1;
-    tlo = p.window && low > 0 ? low / kTile : 0;
+    const int first = max(s.len, 0) - s.n;  // position of the first row
+    tlo = p.window && first >= p.window ? (first - p.window + 1) / kTile : 0;
     nt = max((have + kTile - 1) / kTile - tlo, 1);
     return p.w.KV * nrt * nt;
 }
@@ -767,7 +767,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_attend(const __grid_constan
                 if (lane == 0) mbar_arrive(&br.sempty[sb]);
                 const int tok = t * kTile + tid;
                 if (t * kTile + kTile - 1 > pos_lo || valid != (1 << NP) - 1 ||
-                    (p.window && t * kTile < pos_hi - p.window + 1)) {
+                    (p.window && pos_hi >= p.window && t * kTile <= pos_hi - p.window)) {
                     const bool there = (valid >> page) & 1;
 #pragma unroll
                     for (int r = 0; r < RT; ++r) {
@@ -1194,7 +1194,9 @@ int quantr_kv8_attend_dev(void* out, long long ldo, const void* q, long long ldq
     p.w = kv8_view(pool, tables, batch, layer);
     p.q = q, p.out = out, p.lse = lse, p.ldq = ldq, p.ldo = ldo;
     p.vec = type == QUANTR_TYPE_F32 ? aligned(q, ldq, 4, 16) : aligned(q, ldq, 2, 8);
-    p.H = n_heads, p.G = n_heads / pool->n_kv_heads, p.window = window;
+    p.H = n_heads, p.G = n_heads / pool->n_kv_heads;
+    // A window past every position hides nothing.
+    p.window = window < (long long)tables->max_pages * pool->page_tokens ? window : 0;
     p.inv_g = p.G == 1 ? 0 : (unsigned)(((1ull << 32) + p.G - 1) / p.G);
     p.scale2 = (float)((double)scale * 1.4426950408889634);
     LaunchCfg c;

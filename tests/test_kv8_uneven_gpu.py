@@ -43,3 +43,12 @@ def test_uneven_long_contexts_on_one_workspace(qr_gpu, type_):
             got = attend(qr_gpu, c, q, rows, ws=ws)
             assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     assert qr_gpu.device_status() == 0
+
+
+@pytest.mark.parametrize("window", [5, 1000, 2 ** 31 - 2, 2 ** 31 - 1])
+def test_windows_of_any_size(qr_gpu, window):
+    """A window past every length hides nothing, rows before position 0 or not."""
+    c = Cache(qr_gpu, [3, 300, 1, 0], 2, 64, 64, seed=8)
+    rows = [6, 2, 40, 3]
+    q = query(sum(rows), 4, 64, F32)
+    check(c, q, attend(qr_gpu, c, q, rows, window=window), want_attend(c, q, rows, window=window))
