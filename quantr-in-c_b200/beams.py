@@ -6,6 +6,7 @@ its own where it writes (quantr_kv8_extend_dev), attention reads them all in one
 call (quantr_kv8_attend_dev), and the next tokens are scored with their
 alternatives (quantr_logprobs_dev).  The linear layers are GEMV programs; the
 small elementwise steps between them (norms, RoPE, SwiGLU) are torch operations.
+All of it runs on torch's current stream.
 
 The reference has neither a batch nor beams (its loop is one greedy sequence,
 src/main.c:305-317); the layer is its forward_runtime (src/runtime.c:94-289),
@@ -24,6 +25,11 @@ import torch
 import quantr as qr
 
 F32 = qr.F32
+
+
+def stream():
+    """The stream that the torch operations between the library's calls run on."""
+    return torch.cuda.current_stream().cuda_stream
 
 
 class BeamSearch:
@@ -72,7 +78,7 @@ class BeamSearch:
             self.embd.copy_(torch.from_numpy(model.array("token_embd").view(np.float32)).view(s.vocab_size, s.dim))
         else:
             qr.dequantize_rows_dev(self.embd.data_ptr(), s.dim, self.addr("token_embd"), qr.row_bytes(s.embd_type, s.dim),
-                                   s.embd_type, s.dim, s.vocab_size)
+                                   s.embd_type, s.dim, s.vocab_size, stream=stream())
         # RoPE (src/runtime.c:19-41): the pair at i turns by pos * base^(-i/head_dim).
         i = torch.arange(0, s.q_dim, 2, device=dev, dtype=torch.float64)
         angle = torch.arange(max_len, device=dev)[:, None] * (s.rope_freq_base ** (-i / s.hd))
@@ -123,7 +129,7 @@ class BeamSearch:
         s, ld = self.spec, b["qkv"].shape[1]
         qr.kv8_attend_dev(b["att"].data_ptr(), s.q_dim, b["qkv"].data_ptr(), ld, F32, s.n_heads, self.pool,
                           self.tables[0], batch, layer, s.hd ** -0.5, self.max_len, self.ws.data_ptr(), self.ws.numel(),
-                          window=self.window)
+                          window=self.window, stream=stream())
 
     def forward(self, tokens, pos, batch, T):
         """Logits (T x vocab) of the tokens at positions pos, the last rows of
@@ -134,21 +140,21 @@ class BeamSearch:
         for i in range(s.n_layers):
             qkv, o, h, down = b["prog"][i]
             self._norm(b["xb"], b["x"], self.rms_att[i])
-            qkv.run()
+            qkv.run(stream())
             self._rope(b["qkv"][:, :s.q_dim], pos)
             self._rope(b["qkv"][:, s.q_dim:s.q_dim + s.kv_dim], pos)
             kv = b["qkv"].data_ptr() + 4 * s.q_dim
-            qr.kv8_append_dev(kv, ld, kv + 4 * s.kv_dim, ld, F32, self.pool, self.tables[0], batch, i)
+            qr.kv8_append_dev(kv, ld, kv + 4 * s.kv_dim, ld, F32, self.pool, self.tables[0], batch, i, stream=stream())
             self.attend(b, batch, i)
-            o.run()
+            o.run(stream())
             b["x"] += b["o"]
             self._norm(b["xb"], b["x"], self.rms_ffn[i])
-            h.run()
+            h.run(stream())
             b["h1"].copy_(torch.nn.functional.silu(b["h1"]) * b["h3"])
-            down.run()
+            down.run(stream())
             b["x"] += b["o"]
         self._norm(b["xb"], b["x"], self.rms_final)
-        b["head"].run()
+        b["head"].run(stream())
         return b["logits"]
 
     # ------------------------------------------------------------- the beams --
@@ -157,7 +163,7 @@ class BeamSearch:
         """Beam i goes on from beam pick[i] (-1: ends, and its pages are free
         unless another beam has them)."""
         f = torch.tensor(pick, dtype=torch.int32, device="cuda")
-        qr.kv8_select_dev(self.tables[1], self.tables[0], f.data_ptr(), self.pool)
+        qr.kv8_select_dev(self.tables[1], self.tables[0], f.data_ptr(), self.pool, stream=stream())
         self.tables.reverse()
         self.state.reverse()
         self.lens = [self.lens[p] if p >= 0 else 0 for p in pick]
@@ -166,7 +172,7 @@ class BeamSearch:
         slot = torch.tensor(slots, dtype=torch.int32, device="cuda")
         new = torch.full((len(slots),), n, dtype=torch.int32, device="cuda")
         qr.kv8_extend_dev(self.pool, self.tables[0], slot.data_ptr(), new.data_ptr(), len(slots),
-                          self.ws_pages.data_ptr(), self.ws_pages.numel())
+                          self.ws_pages.data_ptr(), self.ws_pages.numel(), stream=stream())
         for i in slots:
             self.lens[i] += n
 
@@ -178,7 +184,7 @@ class BeamSearch:
         token = torch.full((rows,), -1, dtype=torch.int32, device="cuda") if token is None else token
         qr.logprobs_dev(logits.data_ptr(), logits.stride(0), F32, rows, self.spec.vocab_size, token.data_ptr(),
                         out["logprob"].data_ptr(), out["entropy"].data_ptr(), k, out["ids"].data_ptr(),
-                        out["top"].data_ptr(), None, 0, temperature=temperature)
+                        out["top"].data_ptr(), None, 0, temperature=temperature, stream=stream())
         return out
 
     def prefill(self, prompt):
@@ -243,7 +249,7 @@ class BeamSearch:
         live = torch.empty(1, dtype=torch.int32, device="cuda")
         self.select([beam] + [-1] * (self.beams - 1))
         qr.kv8_compact_dev(self.pool, self.tables[0], None, live.data_ptr(), self.ws_pages.data_ptr(),
-                           self.ws_pages.numel())
+                           self.ws_pages.numel(), stream=stream())
         return int(live)
 
     def close(self):
