@@ -134,27 +134,27 @@ class BeamSearch:
     def forward(self, tokens, pos, batch, T):
         """Logits (T x vocab) of the tokens at positions pos, the last rows of
         the batch's sequences.  Tokens past the batch's are padding."""
-        s, b = self.spec, self._buffers(T)
+        s, b, at = self.spec, self._buffers(T), stream()
         ld = b["qkv"].shape[1]
         b["x"].copy_(self.embd[tokens])
         for i in range(s.n_layers):
             qkv, o, h, down = b["prog"][i]
             self._norm(b["xb"], b["x"], self.rms_att[i])
-            qkv.run(stream())
+            qkv.run(at)
             self._rope(b["qkv"][:, :s.q_dim], pos)
             self._rope(b["qkv"][:, s.q_dim:s.q_dim + s.kv_dim], pos)
             kv = b["qkv"].data_ptr() + 4 * s.q_dim
-            qr.kv8_append_dev(kv, ld, kv + 4 * s.kv_dim, ld, F32, self.pool, self.tables[0], batch, i, stream=stream())
+            qr.kv8_append_dev(kv, ld, kv + 4 * s.kv_dim, ld, F32, self.pool, self.tables[0], batch, i, stream=at)
             self.attend(b, batch, i)
-            o.run(stream())
+            o.run(at)
             b["x"] += b["o"]
             self._norm(b["xb"], b["x"], self.rms_ffn[i])
-            h.run(stream())
+            h.run(at)
             b["h1"].copy_(torch.nn.functional.silu(b["h1"]) * b["h3"])
-            down.run(stream())
+            down.run(at)
             b["x"] += b["o"]
         self._norm(b["xb"], b["x"], self.rms_final)
-        b["head"].run(stream())
+        b["head"].run(at)
         return b["logits"]
 
     # ------------------------------------------------------------- the beams --
@@ -169,12 +169,19 @@ class BeamSearch:
         self.lens = [self.lens[p] if p >= 0 else 0 for p in pick]
 
     def extend(self, slots, n):
+        """Room for n more tokens of the beams in `slots`.  Waits for the
+        device: a beam that it left as it was (its table full, or no page left)
+        must not go on."""
         slot = torch.tensor(slots, dtype=torch.int32, device="cuda")
         new = torch.full((len(slots),), n, dtype=torch.int32, device="cuda")
+        grown = torch.empty_like(slot)
         qr.kv8_extend_dev(self.pool, self.tables[0], slot.data_ptr(), new.data_ptr(), len(slots),
-                          self.ws_pages.data_ptr(), self.ws_pages.numel(), stream=stream())
-        for i in slots:
-            self.lens[i] += n
+                          self.ws_pages.data_ptr(), self.ws_pages.numel(), grown=grown.data_ptr(), stream=stream())
+        done = grown.tolist()
+        for i, ok in zip(slots, done):
+            self.lens[i] += n if ok else 0
+        if not all(done):
+            raise RuntimeError(f"no room for beams {[i for i, ok in zip(slots, done) if not ok]}")
 
     def score(self, logits, rows, k, token=None, temperature=1.0):
         """The k best alternatives of each row with their log probabilities, the

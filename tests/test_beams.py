@@ -110,3 +110,16 @@ def test_all_calls_go_to_the_current_stream(host):
             "logprobs_dev", "dequantize_rows_dev"} <= names
     assert {n for n, s in host.calls if s != SIDE} == set()
     search.close()
+
+
+def test_a_beam_that_could_not_grow_is_told(host):
+    """Lengths follow what the device did, and a beam that it left as it was
+    ends the search with an error instead of wrong positions."""
+    search = beams.BeamSearch(model(), beams=3, max_len=64, page_tokens=32, chunk=16)
+    search.prefill([1] * 10)
+    search.select([0, 0, 0])
+    host.refuse = {1}
+    with pytest.raises(RuntimeError, match="1"):
+        search.step([1, 2, 3])
+    assert search.lens == [11, 10, 11]
+    search.close()

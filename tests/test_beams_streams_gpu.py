@@ -33,3 +33,24 @@ def test_side_stream(qr_gpu):
         assert search.keep(0) == -(-115 // 32)
     assert qr_gpu.device_status() == 0
     search.close()
+
+
+def test_a_pool_that_runs_out_ends_the_search(qr_gpu):
+    """No page left for some beams: an error, lengths as on the device, and the
+    beams that did grow hold their pages."""
+    import beams
+    spec = ms.Spec(dim=256, hidden_dim=256, n_layers=1, n_heads=4, n_kv_heads=4, vocab_size=300, seq_len=96, wtype=8,
+                   head_type=8, embd_type=8)
+    search = beams.BeamSearch(ms.build(spec, seed=3), beams=4, max_len=96, page_tokens=32, chunk=32)
+    search.prefill(ms.prompt(spec, 64)[0])
+    search.select([0, 0, 0, 0])
+    refs = search.state[0][2]
+    free = (refs == 0).nonzero().flatten().tolist()
+    for page in free[2:]:
+        refs[page] = 1  # held by somebody else: two pages left for four beams
+    with pytest.raises(RuntimeError, match=r"\[2, 3\]"):
+        search.step([1, 2, 3, 4])
+    assert search.lens == [65, 65, 64, 64] == search.state[0][1].tolist()
+    assert qr_gpu.device_status() != 0
+    assert qr_gpu.device_status() == 0
+    search.close()
