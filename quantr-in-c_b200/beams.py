@@ -195,20 +195,20 @@ class BeamSearch:
         return out
 
     def prefill(self, prompt):
-        """Writes the prompt into beam 0, `chunk` tokens at a time; the logits of
-        its last token (1 x vocab) and the log probability of each prompt token
-        after the first."""
+        """Writes the prompt into beam 0, behind what it holds, `chunk` tokens at
+        a time; the logits of its last token (1 x vocab) and the log probability
+        of each prompt token after the first."""
         prompt = torch.as_tensor(np.asarray(prompt, np.int32), device="cuda")
-        if not 0 < prompt.numel() <= self.max_len:
-            raise ValueError("the prompt has to have 1 to max_len tokens")
-        T, scores = self.chunk, []
+        T, scores, first = self.chunk, [], self.lens[0]
+        if not 0 < prompt.numel() <= self.max_len - first:
+            raise ValueError("the prompt has to have a token, and max_len has to hold it")
         for at in range(0, prompt.numel(), T):
             part = prompt[at:at + T]
             n = part.numel()
             self.extend([0], n)
             tokens = torch.zeros(T, dtype=torch.long, device="cuda")
             tokens[:n] = part
-            pos = torch.arange(at, at + T, device="cuda").clamp(max=self.max_len - 1)
+            pos = torch.arange(first + at, first + at + T, device="cuda").clamp(max=self.max_len - 1)
             batch = qr.Kv8Batch(None, None, 1, n)
             logits = self.forward(tokens, pos, batch, T)
             follow = torch.full((n,), -1, dtype=torch.int32, device="cuda")

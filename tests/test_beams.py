@@ -123,3 +123,15 @@ def test_a_beam_that_could_not_grow_is_told(host):
         search.step([1, 2, 3])
     assert search.lens == [11, 10, 11]
     search.close()
+
+
+def test_a_prompt_behind_a_prompt_has_to_fit(host):
+    search = beams.BeamSearch(model(), beams=2, max_len=64, page_tokens=32, chunk=16)
+    search.prefill([1] * 40)
+    done = len(host.calls)
+    with pytest.raises(ValueError):
+        search.prefill([1] * 25)
+    assert search.lens == [40, 0] and len(host.calls) == done
+    search.prefill([1] * 24)
+    assert search.lens == [64, 0]
+    search.close()

@@ -54,3 +54,26 @@ def test_a_pool_that_runs_out_ends_the_search(qr_gpu):
     assert qr_gpu.device_status() != 0
     assert qr_gpu.device_status() == 0
     search.close()
+
+
+def test_a_prompt_in_two_parts(qr_gpu):
+    """A second prefill goes on behind the first: the logits of a prompt given
+    in two parts are those of the whole.  (Its second part begins a page, so the
+    cache holds the same codes: what is left is rounding of the activations to 8
+    bits, 2^-7 of a block's largest.)"""
+    import beams
+    spec = ms.Spec(dim=256, hidden_dim=512, n_layers=2, n_heads=8, n_kv_heads=2, vocab_size=600, seq_len=192, wtype=8,
+                   head_type=8, embd_type=8)
+    model = ms.build(spec, seed=5)
+    prompt = ms.prompt(spec, 96)[0]
+    got = []
+    for parts in ([prompt], [prompt[:64], prompt[64:]]):
+        search = beams.BeamSearch(model, beams=2, max_len=192, page_tokens=32, chunk=32)
+        for p in parts:
+            logits, scores = search.prefill(p)
+        got.append((logits.clone(), scores[-31:].clone()))
+        assert search.lens == [96, 0]
+        search.close()
+    for a, b in zip(*got):
+        assert float((a - b).abs().max()) <= 2.0 ** -7 * max(1.0, float(b.abs().max()))
+    assert qr_gpu.device_status() == 0
