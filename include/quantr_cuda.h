@@ -552,6 +552,9 @@ int quantr_kv8_read_dev(void* k, long long ldk, void* v, long long ldv, uint32_t
  * q and out have `type` (F32/F16/BF16).  A row that sees nothing (position
  * below 0, all of its pages missing) gives out = 0, lse = -inf; a page that is
  * missing counts as masked.  A query or a scale that is not finite gives NaN.
+ * Whatever the type, a query element is kept to 2^-23 of the largest of its row
+ * and head (all are 0 where that is below 3e-32), a weight to 2^-24 of the
+ * largest of its page; sums and statistics are fp32, results rounded once.
  * max_len (>= 0) is the longest sequence expected; neither the split of long
  * sequences over the GPU nor the workspace depends on it, since the lengths are
  * read on the device.  The workspace must be 256-byte aligned and its first 4096

@@ -3,23 +3,27 @@
 //
 // Mathematics.  The cache's codes are the tensor cores' own 8-bit integers, so
 // the products are integer products (tcgen05.mma kind::i8, int32 sums, exact):
-// a query row is written in fixed point as `DG` signed 8-bit digits relative to
-// its largest magnitude, and a softmax weight as `DG` unsigned ones relative to
+// a query row is written in fixed point as three signed 8-bit digits relative to
+// its largest magnitude, and a softmax weight as three unsigned ones relative to
 // the largest weight of its page, and each digit is a column of the product's
 // second operand:
 //
 //   S^T (128 tokens x columns) = K (tokens x hd) . Qdigits^T
 //   O^T (hd x columns)         = V^T (hd x tokens) . Wdigits^T      (per page)
 //
-// fp32 inputs take three digits (24 and 23 bits: no less than an fp32 product
-// of the row's largest element keeps), 16-bit ones two: the step is a power of
-// two near 2^-15 of the row's largest element, so that fp16 elements within
-// 2^-4 and bf16 elements within 2^-7 of it are exact and smaller ones lose
-// 2^-16 of it.  K and V go from memory to the tensor cores without one
-// conversion.  Weights relative to their page, not to the running maximum:
-// the digits then cost a page at most 2^-24 (2^-17) of its own mass, wherever
-// the maximum of a long row lies, and a page has one scale, which the join
-// applies once per page instead of once per token.
+// These are the only roundings that the integers add, the same for all types of
+// queries: an element is kept to 2^-23 of its row's largest (fp16 elements within
+// 2^-11 and bf16 ones within 2^-14 of it exactly), a weight to 2^-24 of its page's
+// largest, so a page's output is off by up to page_tokens * 2^-24 of that weight
+// times its largest value, and the weights' sum adds the same numbers.
+// Two digits for 16-bit types would save 1 to 12 % (64-token chunks 53.1 -> 47.0
+// us, 512 tokens 271 -> 251, long contexts 88.4 -> 87.0), but beside a token that
+// has most of the weight they lose all others below 2^-17 of it, and queries with
+// one large element lose their small ones.  K and V go from memory to the tensor
+// cores without one conversion.  Weights are relative to their page, not to the
+// running maximum: what the digits cost a page does not depend on where the
+// maximum of a long row lies, and a page has one scale, which the join applies
+// once per page instead of once per token.
 //
 // Work is shared out in (sequence, KV head, row tile of up to 16 rows) x
 // 128-token tiles; see walk_begin.  A row tile that several CTAs share is joined
@@ -28,21 +32,22 @@
 //
 // Roles (320 threads, two CTAs per SM): warps 0-3 softmax (thread = token), 4-7
 // join (thread = output element), 8 copies (TMA, up to 6 stages ahead), 9 issues
-// the MMAs.  S has two TMEM buffers, so a tile's scores are computed while the
-// tile before is weighted, and its outputs while the next is scored.
+// the MMAs.  S has two TMEM buffers (one under 16 rows and pages of 32 tokens), so
+// a tile's scores are computed while the tile before is weighted, and its outputs
+// while the next is scored.
 //
 // What bounds it, and what it measured (B200, 6.54 TB/s copy; launches back to
 // back in a graph, inputs in rotation):
 //   8 sequences of 200 to 262 thousand tokens, 32/4 heads of 128, bf16: 1.87 GB
-//     in 292 us, 6.4 TB/s: memory.  4 of 100 to 131 thousand (459 MB): 86.7 us,
-//     5.3 TB/s; the 16 us above the copy rate are launch, start (length, page
+//     in 285 us, 6.5 TB/s: memory.  4 of 100 to 131 thousand (459 MB): 88.4 us,
+//     5.2 TB/s; the 18 us above the copy rate are launch, start (length, page
 //     entry and keys are loads that wait for one another) and the join of the
 //     18 to 20 CTAs that share a row tile.
 //   64 sequences of 640 to 1152 tokens, fp32 (61 MB): 20.0 us, 3.1 TB/s; the start
 //     and the longest CTA's tiles, one after the other.
 //   1 sequence of 513 tokens: 8.6 us; latency, of one tile and the join of five.
-//   6 prompt chunks of 64 tokens (2.2 GFLOP): 47.1 us; issue slots are 53 % used,
-//     the tensor pipe 4 %.  512 tokens after 3584 (32 GFLOP): 254 us; a tile takes
+//   6 prompt chunks of 64 tokens (2.2 GFLOP): 53.1 us; issue slots are 53 % used,
+//     the tensor pipe 4 %.  512 tokens after 3584 (32 GFLOP): 271 us; a tile takes
 //     4000 cycles (clock readings), nearly all in the softmax warps, of which two
 //     CTAs per SM keep two in flight.
 // Tried and not kept, each beside what it was at that step, in us: one reference
@@ -361,13 +366,11 @@ __device__ __forceinline__ void walk_next(const AttendParams& p, Walk& k)
 
 // ------------------------------------------------------------- shared memory --
 
-// Digits of queries and weights: three for fp32, two for 16-bit types.
-template <typename T>
-constexpr int digits = sizeof(T) == 4 ? 3 : 2;
+constexpr int kDigits = 3;  // of queries and weights
 
-template <int DG, int RT>
+template <int RT>
 struct Shape {
-    static constexpr int N = (DG * RT + 15) / 16 * 16;
+    static constexpr int N = (kDigits * RT + 15) / 16 * 16;
     static constexpr uint32_t kPBytes = N * 128;
 };
 
@@ -423,20 +426,18 @@ __device__ __forceinline__ void load_rows(const float* src, float (&x)[N])
 // magnitude, so two of them make one int32.  Conversions are slow here (they
 // share a quarter-rate pipe with ex2): the third digit takes 1.5 * 2^23 in its
 // integer, which is a float's bit pattern.
-template <int DG, int C>
-__device__ __forceinline__ float digits_value(const int (&c)[DG][C], int r)
+template <int C>
+__device__ __forceinline__ float digits_value(const int (&c)[kDigits][C], int r)
 {
     const float hi = (float)(c[0][r] * 256 + c[1][r]);
-    if constexpr (DG == 2) return hi;
-    else return fmaf(hi, 256.0f, __int_as_float(0x4b400000 + c[2][r]) - 12582912.0f);
+    return fmaf(hi, 256.0f, __int_as_float(0x4b400000 + c[2][r]) - 12582912.0f);
 }
 
 template <typename T, int RT, int HDW>
 __global__ void __launch_bounds__(kThreads, 2) k_kv8_attend(const __grid_constant__ AttendParams p)
 {
-    constexpr int DG = digits<T>;
-    constexpr int N = Shape<DG, RT>::N;
-    constexpr uint32_t kStage = kTile * HDW, kPBytes = Shape<DG, RT>::kPBytes;
+    constexpr int N = Shape<RT>::N;
+    constexpr uint32_t kStage = kTile * HDW, kPBytes = Shape<RT>::kPBytes;
     constexpr uint32_t kSw = HDW == 128 ? 2u : 4u;  // 128- or 64-byte swizzle
     extern __shared__ uint8_t raw[];
     uint8_t* sm = reinterpret_cast<uint8_t*>(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
@@ -651,7 +652,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_attend(const __grid_constan
         const int tid = threadIdx.x, page = tid >> p.w.lgP;
         int sb = 0, su = 0, pb = 0, pu = 0, mt = 0, mu = 0, seg = 0;
         const uint32_t tm = tm_s + ((uint32_t)warp << 21);
-        constexpr float kQMax = DG == 3 ? 8323072.0f : 32512.0f;  // 127 * 256^(DG-1)
+        constexpr float kQMax = 8323072.0f;  // 127 * 256^2
         // Query rows warp, warp + 4, ... of a row tile; lane l has 4 elements.
         constexpr int kRows = RT / 4;
         auto load_q = [&](const Seg& k, float (&x)[kRows][4]) {
@@ -698,7 +699,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_attend(const __grid_constan
                 // in range.  Below 3e-32 (no power of two for it) rows count as 0.
                 float inv = 0.0f, step = 0.0f;
                 if (fine && top > 3e-32f) {
-                    const int ex = 252 + 8 * DG - (int)(__float_as_uint(top) >> 23);
+                    const int ex = 252 + 8 * kDigits - (int)(__float_as_uint(top) >> 23);
                     inv = __uint_as_float((uint32_t)ex << 23);
                     if (top * inv > kQMax) inv *= 0.5f;
                     step = 1.0f / inv;
@@ -708,7 +709,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_attend(const __grid_constan
                 for (int j = 0; j < 4; ++j) {
                     int v = fine ? __float2int_rn(x[j] * inv) : 0;
 #pragma unroll
-                    for (int d = DG - 1; d >= 0; --d) {
+                    for (int d = kDigits - 1; d >= 0; --d) {
                         const int lo = (int)(int8_t)v;
                         dig[d] |= (uint32_t)(lo & 255) << (8 * j);
                         v = (v - lo) >> 8;
@@ -716,7 +717,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_attend(const __grid_constan
                 }
                 if (e < HDW) {
 #pragma unroll
-                    for (int d = 0; d < DG; ++d) {
+                    for (int d = 0; d < kDigits; ++d) {
                         const int n = d * RT + r;
                         const int sw = HDW == 128 ? (n & 7) : ((n >> 1) & 3);
                         *reinterpret_cast<uint32_t*>(qsm + n * HDW + ((((e >> 4) ^ sw) << 4) | (e & 15))) = dig[d];
@@ -750,9 +751,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_attend(const __grid_constan
 #pragma unroll
                 for (int r0 = 0; r0 < RT; r0 += (RT < 8 ? RT : 8)) {
                     constexpr int C = RT < 8 ? RT : 8;
-                    int c[DG][C];
+                    int c[kDigits][C];
 #pragma unroll
-                    for (int d = 0; d < DG; ++d) {
+                    for (int d = 0; d < kDigits; ++d) {
                         if constexpr (C == 8) tmem_ld8(tm + sb * N + d * RT + r0, c[d]);
                         else tmem_ld4(tm + sb * N + d * RT + r0, c[d]);
                     }
@@ -760,7 +761,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_attend(const __grid_constan
                     load_rows<C>(&z.qscale[sg][r0], qs);
                     tmem_wait();
 #pragma unroll
-                    for (int r = 0; r < C; ++r) x[r0 + r] = digits_value<DG, C>(c, r) * (qs[r] * ks);
+                    for (int r = 0; r < C; ++r) x[r0 + r] = digits_value<C>(c, r) * (qs[r] * ks);
                 }
                 fence_before();
                 __syncwarp();
@@ -800,22 +801,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_attend(const __grid_constan
                 uint8_t* pt = psm + pb * kPBytes + (tid & 15);
 #pragma unroll
                 for (int r = 0; r < RT; ++r) {
-                    // Weight of the token relative to its page's largest.  1 + w
-                    // holds w to 23 bits in its low bits, 128 + w to 16.  With
-                    // two digits the largest weight is 65535/65536.
+                    // Weight of the token relative to its page's largest: 1 + w
+                    // holds it to 23 bits in its low bits.
                     const float ref = mx[r] == -INFINITY ? 0.0f : mx[r];
-                    const float w = ex2(DG == 3 ? x[r] - ref : x[r] - ref - 2.2013990e-5f);
-                    const uint32_t u = __float_as_uint(1.0f + w);
-                    const uint32_t d = DG == 3 ? u : __float_as_uint(128.0f + w);
+                    const uint32_t u = __float_as_uint(1.0f + ex2(x[r] - ref));
                     auto put = [&](int n, uint32_t v) { pt[n * 128 + (((tid >> 4) ^ (n & 7)) << 4)] = (uint8_t)v; };
-                    if constexpr (DG == 3) {
-                        put(r, (d >> 16) - 0x80);
-                        put(r + RT, d >> 8);
-                        put(r + 2 * RT, d);
-                    } else {
-                        put(r, d >> 8);
-                        put(r + RT, d);
-                    }
+                    put(r, (u >> 16) - 0x80);
+                    put(r + RT, u >> 8);
+                    put(r + 2 * RT, u);
                     // u - 0x3f800000 per lane
                     sum[r] = __uint_as_float(__reduce_add_sync(~0u, u));
                 }
@@ -839,7 +832,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_attend(const __grid_constan
         const uint32_t tm = tm_o + ((uint32_t)w4 << 21);
         int sb = 0, su = 0, ob = 0, ou = 0, meets = 0;
         bool ok = true;
-        constexpr float kUnit = DG == 3 ? 1.0f / 8388608.0f : 1.0f / 65536.0f;
+        constexpr float kUnit = 1.0f / 8388608.0f;
         constexpr size_t kPart = RT * 130;
         constexpr int kSets = RT <= 8 ? 1 : RT / 8, kSet = RT < 8 ? RT : 8;
         const int me = blockIdx.x;
@@ -853,7 +846,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_attend(const __grid_constan
             lse = row * p.H + hq;
         };
         auto lse_of = [&](float m, float l) {
-            return m == -INFINITY ? m : (m + log2f(l) + (DG == 3 ? 0.0f : 2.2013990e-5f)) * 0.693147180559945f;
+            return m == -INFINITY ? m : (m + log2f(l)) * 0.693147180559945f;
         };
         // Counts this CTA in; true in all join threads if it is the last of n,
         // and then the others' parts can be read.
@@ -900,7 +893,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_attend(const __grid_constan
                     mn = max_nan(mn, __shfl_xor_sync(~0u, mn, 8));
                     mn = max_nan(mn, __shfl_xor_sync(~0u, mn, 16));
                     const float ref = mn == -INFINITY ? 0.0f : mn, f = ex2(mp - ref), a = ex2(m_run[i] - ref);
-                    float l = sum * (1.0f / 8388608.0f) * f;
+                    float l = sum * kUnit * f;
                     l += __shfl_xor_sync(~0u, l, 8);
                     l += __shfl_xor_sync(~0u, l, 16);
                     l_run[i] = fmaf(l_run[i], a, l);
@@ -925,9 +918,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_attend(const __grid_constan
 #pragma unroll
                     for (int r0 = 0; r0 < RT; r0 += (RT < 8 ? RT : 8)) {
                         constexpr int C = RT < 8 ? RT : 8;
-                        int c[DG][C];
+                        int c[kDigits][C];
 #pragma unroll
-                        for (int d = 0; d < DG; ++d) {
+                        for (int d = 0; d < kDigits; ++d) {
                             if constexpr (C == 8) tmem_ld8(tm + (ob * NP + j) * N + d * RT + r0, c[d]);
                             else tmem_ld4(tm + (ob * NP + j) * N + d * RT + r0, c[d]);
                         }
@@ -936,7 +929,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_attend(const __grid_constan
                         tmem_wait();
 #pragma unroll
                         for (int r = 0; r < C; ++r) {
-                            o[r0 + r] = fmaf(digits_value<DG, C>(c, r), w[r], o[r0 + r]);
+                            o[r0 + r] = fmaf(digits_value<C>(c, r), w[r], o[r0 + r]);
                         }
                     }
                 }
@@ -1077,32 +1070,33 @@ int pick_rt(const quantr_kv8_batch* b, int G)
 }
 
 struct Plan {
-    int stages, nS, nO, cols, occ, grid;
+    int stages, nS, nO, cols, grid;
     size_t smem;
 };
 
-template <int DG, int RT, int HDW>
+template <int RT, int HDW>
 Plan make_plan(int lgP)
 {
-    constexpr int N = Shape<DG, RT>::N;
+    constexpr int N = Shape<RT>::N;
+    static_assert(N * (1 + kTile / 32) <= 256, "half of an SM's TMEM holds a buffer of either");
     const int NP = kTile >> lgP;
     Plan r{};
-    // Two buffers of scores and of outputs where 256 TMEM columns hold them
-    // (two CTAs per SM), else fewer outputs, else one CTA per SM.
-    const int tries[4][3] = {{2, 2, 256}, {2, 1, 256}, {2, 1, 512}, {1, 1, 512}};
+    // Two buffers of scores and of outputs where 256 TMEM columns hold them, half
+    // an SM's (two CTAs per SM); else one of outputs, else one of either (rows of
+    // 16 over pages of 32: 64-token chunks 53 us, 70 with one CTA per SM and two
+    // buffers of scores).
+    const int tries[3][2] = {{2, 2}, {2, 1}, {1, 1}};
     for (auto& t : tries) {
         r.nS = t[0], r.nO = t[1];
-        const int need = N * (t[0] + t[1] * NP);
-        if (need > t[2]) continue;
-        for (r.cols = 32; r.cols < need;) r.cols *= 2;
-        r.occ = r.cols <= 256 ? 2 : 1;
-        break;
+        r.cols = 32;
+        while (r.cols < N * (t[0] + t[1] * NP)) r.cols *= 2;
+        if (r.cols <= 256) break;
     }
-    const size_t fixed = 1024 + 2 * Shape<DG, RT>::kPBytes + N * HDW + sizeof(Small<RT>);
-    const size_t room = (r.occ == 2 ? 113 : 226) * 1024;
+    const size_t fixed = 1024 + 2 * Shape<RT>::kPBytes + N * HDW + sizeof(Small<RT>);
+    const size_t room = 113 * 1024;
     r.stages = (int)std::min<size_t>(kMaxStages, (room - fixed) / (2 * kTile * HDW));
     r.smem = fixed + (size_t)r.stages * 2 * kTile * HDW;
-    r.grid = std::min(r.occ * device_sm_count(), kJoinCtas);
+    r.grid = std::min(2 * device_sm_count(), kJoinCtas);
     return r;
 }
 
@@ -1129,7 +1123,7 @@ bool encode_map(CUtensorMap* map, const void* base, const quantr_kv8_pool* p, in
 template <typename T, int RT, int HDW>
 cudaError_t run(AttendParams& p, const quantr_kv8_pool* pool, void* ws, const LaunchCfg& c)
 {
-    const Plan r = make_plan<digits<T>, RT, HDW>(p.w.lgP);
+    const Plan r = make_plan<RT, HDW>(p.w.lgP);
     static int configured = -1;
     cudaError_t e = ensure_smem_attr(k_kv8_attend<T, RT, HDW>, 227 * 1024, configured);
     if (e != cudaSuccess) return e;
