@@ -482,8 +482,8 @@ int quantr_gemv_noalloc_dev(float* out, long long ldo, const float* x, long long
  * multiples of their elements' size (QUANTR_ERR_BAD_ARG if not).  Every call is
  * asynchronous on `stream`, allocates nothing and can be captured (the first
  * call on a device allocates its error word: make it before any capture).
- * What only the device can see - a slot or page id out of range, a table too
- * short for a length, an empty pool - is skipped as each call describes and
+ * What only the device can see - a slot or page id out of range, a length below
+ * 0, a table too short for one, an empty pool - is skipped as each call describes and
  * reported by quantr_gpu_device_status as QUANTR_ERR_PAGES.
  * -------------------------------------------------------------------------*/
 

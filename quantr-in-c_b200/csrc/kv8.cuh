@@ -124,8 +124,9 @@ __device__ __forceinline__ void kv8_fault(int* err)
     if (err) atomicCAS(err, (int)DEV_OK, (int)DEV_ERR_PAGES);
 }
 
-// One sequence of the batch: its table row (null: no such slot), its length,
-// its rows row0 .. row0+n-1, the first of which stands at position len - n.
+// One sequence of the batch: its table row (null: no such slot), its length (0
+// where it is below), its rows row0 .. row0+n-1, the first of which stands at
+// position len - n.
 struct Kv8Seq {
     const int* pages;
     int len, n, row0;
@@ -151,6 +152,7 @@ __device__ __forceinline__ Kv8Seq kv8_seq(const Kv8View& w, int b)
     s.pages = w.table + (size_t)slot * w.max_pages;
     s.len = w.lens[slot];
     if (s.len < 0 || (long long)s.len > (long long)w.max_pages * w.P) kv8_fault(w.err);
+    s.len = max(s.len, 0);
     return s;
 }
 

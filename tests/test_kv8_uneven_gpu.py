@@ -7,7 +7,7 @@ import pytest
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
-from test_kv8_gpu import BF16, F32, Cache, attend, check, query, want_attend  # noqa: E402
+from test_kv8_gpu import BF16, ERR_PAGES, F32, Cache, attend, check, query, want_attend  # noqa: E402
 
 SHAPES = [
     # KV, G, lens: on 296 CTAs the last group of one row tile is one CTA, which
@@ -52,3 +52,26 @@ def test_windows_of_any_size(qr_gpu, window):
     rows = [6, 2, 40, 3]
     q = query(sum(rows), 4, 64, F32)
     check(c, q, attend(qr_gpu, c, q, rows, window=window), want_attend(c, q, rows, window=window))
+
+
+@pytest.mark.parametrize("length", [-1, -70, -2 ** 31 + 1, -2 ** 31])
+def test_lengths_below_zero_are_empty(qr_gpu, length):
+    """A length below 0 is an empty sequence to every call, and is reported."""
+    c = Cache(qr_gpu, [100, 70], 2, 32, 32, seed=9)
+    keys, used = c.k.clone(), c.table[1].clone()
+    c.lens[0] = length
+    q = query(5, 4, 32, F32)
+    out, lse = attend(qr_gpu, c, q, [3, 2])
+    assert bool((out[:3] == 0).all()) and bool(torch.isneginf(lse[:3]).all()) and bool(torch.isfinite(lse[3:]).all())
+    assert qr_gpu.device_status() == ERR_PAGES
+    b = qr_gpu.Kv8Batch(None, None, 2, 3)
+    rows = torch.full((2, 6, 2, 32), 7.0, device="cuda")
+    qr_gpu.kv8_read_dev(rows[0].data_ptr(), 64, rows[1].data_ptr(), 64, F32, c.pool, c.tables, b, 0)
+    torch.cuda.synchronize()
+    assert bool((rows[:, :3] == 0).all()) and bool((rows[:, 3:] != 7).all())
+    assert qr_gpu.device_status() == ERR_PAGES
+    qr_gpu.kv8_append_dev(rows[0].data_ptr(), 64, rows[1].data_ptr(), 64, F32, c.pool, c.tables, b, 0)
+    torch.cuda.synchronize()
+    others = [p for p in range(c.k.shape[0]) if p not in used.tolist()]
+    assert torch.equal(c.k[others], keys[others])
+    assert qr_gpu.device_status() == ERR_PAGES
