@@ -229,15 +229,16 @@ class BeamSearch:
     def run(self, prompt, steps):
         """The `beams` best continuations of `steps` tokens: int32[beams, steps]
         and the sums of their log probabilities, best first."""
-        B, V = self.beams, self.spec.vocab_size
+        B = k = self.beams
+        if steps < 1:
+            raise ValueError("at least one step")
+        if self.spec.vocab_size < B:
+            raise ValueError("more beams than tokens")
         self.select([-1] * B)
         logits, _ = self.prefill(prompt)
-        k = min(B, V)
         first = self.score(logits, 1, k)
-        tokens = first["ids"].cpu().numpy().T.astype(np.int32)  # (k, 1)
+        tokens = first["ids"].cpu().numpy().T.astype(np.int32)  # (B, 1)
         scores = first["top"].cpu().numpy()[0].astype(np.float64)
-        if k < B:
-            raise ValueError("more beams than tokens")
         self.select([0] * B)
         for _ in range(steps - 1):
             got = self.score(self.step(tokens[:, -1]), B, k)

@@ -135,3 +135,18 @@ def test_a_prompt_behind_a_prompt_has_to_fit(host):
     search.prefill([1] * 24)
     assert search.lens == [64, 0]
     search.close()
+
+
+@pytest.mark.parametrize("beams_,steps", [(2, 0), (2, -3), (20, 4)])
+def test_run_refuses_before_it_begins(host, beams_, steps):
+    """No steps, or more beams than tokens to begin with: nothing is launched and
+    the cache stays as it is."""
+    spec = ms.Spec(dim=256, hidden_dim=256, n_layers=1, n_heads=4, n_kv_heads=2, vocab_size=16, seq_len=64, wtype=8,
+                   head_type=8, embd_type=8)
+    search = beams.BeamSearch(ms.build(spec, seed=1), beams=beams_, max_len=64, page_tokens=32, chunk=16)
+    search.prefill([1] * 10)
+    done = len(host.calls)
+    with pytest.raises(ValueError):
+        search.run([1, 2, 3], steps)
+    assert len(host.calls) == done and search.lens[0] == 10
+    search.close()
