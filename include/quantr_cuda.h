@@ -582,7 +582,8 @@ int quantr_kv8_select_dev(const quantr_kv8_tables* to, const quantr_kv8_tables* 
  * several sequences that share it, the last one in the batch keeps it if
  * nobody else does); then adds n_new to lens.  grown[b] (optional) = 1, or 0
  * where the sequence was left as it was: its table is too short, or the pages
- * ran out (then for every later sequence that needs one too). */
+ * ran out (then for every later sequence that needs one too).  The workspace,
+ * compact's too, is 256-byte aligned; its size goes by the pool alone. */
 size_t quantr_kv8_pages_workspace_bytes(const quantr_kv8_pool* pool, const quantr_kv8_tables* tables);
 int quantr_kv8_extend_dev(const quantr_kv8_pool* pool, const quantr_kv8_tables* tables, const int* slot,
                           const int* n_new, int B, int* grown, void* workspace, size_t workspace_bytes,

@@ -125,8 +125,9 @@ struct AppendArgs {
 // thread holds its vectors of the new rows from the maximum to the codes, so
 // the rows are read once, and a chain of three dependent loads (length, page,
 // old scale) is all that a single token waits for.  64 sequences' tokens (fp32, 4
-// heads of 128): 2.2 us, latency.  8 prompts of up to 2048 tokens (bf16, 46 MB):
-// 13.2 us, 3.5 TB/s: that chain, and conversions (issue slots 66 % used).
+// heads of 128): 2.3 us, latency.  8 prompts of up to 2048 tokens (bf16, 46 MB):
+// 11.5 us, 3.9 TB/s: that chain, a barrier and the stores one after another, and
+// conversions beside them (issue slots 82 % used while a CTA is there).
 template <typename T>
 __global__ void __launch_bounds__(kAppendMax) k_kv8_append(const AppendArgs a)
 {
@@ -253,7 +254,7 @@ __device__ __forceinline__ void store8(T* p, bool vec, const float (&x)[8])
 
 // One CTA per (sequence, page, head, k or v), like the append; a thread takes
 // eight codes at a time.  The same prompts to fp32 (76 MB, most of it written):
-// 15.0 us, 5.1 TB/s: memory.  CTA m = 0 of a sequence also zeroes its rows before
+// 15.1 us, 5.0 TB/s: memory.  CTA m = 0 of a sequence also zeroes its rows before
 // position 0.
 template <typename T>
 __global__ void __launch_bounds__(kReadThreads) k_kv8_read(const ReadArgs a)

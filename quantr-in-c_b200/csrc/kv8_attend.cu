@@ -39,17 +39,20 @@
 // What bounds it, and what it measured (B200, 6.54 TB/s copy; launches back to
 // back in a graph, inputs in rotation):
 //   8 sequences of 200 to 262 thousand tokens, 32/4 heads of 128, bf16: 1.87 GB
-//     in 285 us, 6.5 TB/s: memory.  4 of 100 to 131 thousand (459 MB): 88.4 us,
+//     in 286 us, 6.5 TB/s: memory.  4 of 100 to 131 thousand (459 MB): 88.4 us,
 //     5.2 TB/s; the 18 us above the copy rate are launch, start (length, page
 //     entry and keys are loads that wait for one another) and the join of the
 //     18 to 20 CTAs that share a row tile.
 //   64 sequences of 640 to 1152 tokens, fp32 (61 MB): 20.0 us, 3.1 TB/s; the start
 //     and the longest CTA's tiles, one after the other.
 //   1 sequence of 513 tokens: 8.6 us; latency, of one tile and the join of five.
-//   6 prompt chunks of 64 tokens (2.2 GFLOP): 53.1 us; issue slots are 53 % used,
-//     the tensor pipe 4 %.  512 tokens after 3584 (32 GFLOP): 271 us; a tile takes
-//     4000 cycles (clock readings), nearly all in the softmax warps, of which two
-//     CTAs per SM keep two in flight.
+//   6 prompt chunks of 64 tokens (2.2 GFLOP): 52.9 us.  512 tokens after 3584 (32
+//     GFLOP): 270 us.  A tile takes some 4000 cycles (clock readings, with two
+//     digits), nearly all in the softmax warps, of which two CTAs per SM keep two
+//     in flight: a thread has one token and goes through 16 rows, each with two
+//     warp-wide reductions and stores of single bytes.  No pipe is full (issue
+//     slots 55 to 58 %, tensor 5 to 9 %, ex2 and conversions 6 to 7 %); the kernels
+//     of 16 rows spill 36 to 116 bytes at their 96 registers.
 // Tried and not kept, each beside what it was at that step, in us: one reference
 // weight per warp's 32 tokens instead of per page (no exchange between warps, but
 // four outputs per tile to join: long contexts 94 -> 103); scoring a tile ahead
@@ -70,7 +73,11 @@ constexpr int kThreads = 320;
 constexpr int kTile = 128;     // tokens per tile
 constexpr int kMeta = 16;      // rings of the segments, and of the tiles' page scales
 constexpr int kMaxStages = 6;
-constexpr int kSlack = 5;      // tiles that sharing out by row tiles may cost the longest CTA
+// Tiles that sharing out by row tiles may cost the longest CTA.  With 0, 64 sequences
+// of 640 to 1152 tokens take 26.5 us instead of 20.0; with 2, 16 of 1000 to 2000
+// with 16 KV heads 27.2 instead of 24.5; with 12, 20 of 2000 to 8000 36.7 instead
+// of 32.8; always by row tiles, 8 of 500 to 100,000 75.5 instead of 54.6.
+constexpr int kSlack = 5;
 
 struct AttendParams {
     CUtensorMap kmap, vmap;
@@ -243,7 +250,10 @@ __device__ __forceinline__ int quotient(int a, int b)
 // This CTA's part of the work and its first segment.  Two ways to share it out:
 //   by row tiles, where there are no more of them than CTAs and their lengths
 //   differ little: a row tile has `per` CTAs, each with one run of its tiles
-//   (at least sqrt(nt/12): a part costs the join about a twelfth of a tile);
+//   (at least sqrt(nt/12): a part costs the join about a twelfth of a tile.  With
+//   a third, one sequence of 16,384 tokens takes 19.8 us instead of 18.7 and one
+//   of 131,072 40.9 instead of 35.6; with a 48th, 16.8 and 35.7, but one of 4096
+//   14.7 instead of 12.4);
 //   by tiles, else: equal runs of the flat list of all tiles.
 // Lane l looks at the sequences 32 i + l.
 template <int RT>

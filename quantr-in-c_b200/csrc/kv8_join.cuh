@@ -24,6 +24,9 @@
 
 namespace qr {
 
+// (Groups from 17 parts up: one sequence of 16,384 tokens 19.5 us instead of 18.7,
+// 8 of 500 to 100,000 56.5 instead of 54.6.  Groups of 32: one of 131,072 39.0
+// instead of 35.6.)
 constexpr int kJoinAll = 32;
 constexpr int kJoinGroup = 16;
 constexpr int kJoinCtas = 512;  // most CTAs; 2 * kJoinCtas counters, zero between calls

@@ -5,24 +5,30 @@
 // maximum m of its logits, s = sum 2^(c(x-m)) and e = sum 2^(c(x-m)) c(x-m);
 // joined over the row,
 //   lse = m/temperature + ln s,  entropy = ln2 (log2 s - e/s).
+// A thread's exponents are c x - r with r = c m rounded, one instruction for two;
+// what the rounding leaves out (lo = c m - r) is part of its sums, and taken out
+// of them where they meet sums about another maximum.  Where lo would be large
+// (maxima millions of temperatures from 0) they are c (x - m).
 // One pass: each logit is read once, whatever is asked for.
 //
 // Alternatives cost the pass nothing but a store: a thread keeps the maximum of
 // each group of its elements, which the softmax needs anyway.  Then a threshold
 // that k elements of the row reach at least (the k-th largest of every warp's
 // few largest thread maxima), and only the groups that reach it are read again,
-// about k of thousands.  Their elements are ranked as 64-bit keys (logit, ~id), all different: ties go to
-// the lower id, and the order of the threads does not matter.
+// about k of thousands.  Their elements are ranked as 64-bit keys (logit, ~id), all
+// different: ties go to the lower id, and the order of the threads does not
+// matter.
 //
 // A row is one CTA, or a cluster of up to 8 where there are few rows, joined
 // through distributed shared memory.
 //
 // What bounds it, and what it measured (B200, 6.54 TB/s copy): 2047 rows of
-// 151,936 bf16 logits (622 MB), 4 alternatives: 122 us, 5.1 TB/s; without them 105
-// to 108 (an ex2 per logit beside the conversions); 1024 fp32 rows without them,
-// the same bytes, 95, 6.6 TB/s: memory.  64 fp32 rows (39 MB), 20 alternatives:
-// 15.0 us; 10.8 without: a row's end is a chain of a threshold, a second read and
-// a ranking.  One row of 32,000: 6.4 us, 3.3 without alternatives: latency.
+// 151,936 bf16 logits (622 MB), 4 alternatives: 123 us, 5.1 TB/s; without them 106
+// (an ex2 per logit beside the conversions, and 3.46 waves of CTAs); 1024 fp32
+// rows without them, the same bytes, 95, 6.5 TB/s: memory.  64 fp32 rows (39 MB),
+// 20 alternatives: 15.0 us; 10.8 without: a row's end is a chain of a threshold, a
+// second read and a ranking.  One row of 32,000: 6.4 to 6.6 us, 3.4 without
+// alternatives: latency.
 // Tried and not kept: rings of bulk copies in shared memory (without
 // alternatives 146 -> 187 us at that step), CTAs that stay and fetch the next row
 // during a row's end (no change), 128 threads per CTA (prompt 123 -> 145).
@@ -48,7 +54,7 @@ typedef unsigned long long u64;
 struct LpArgs {
     const void* x;
     long long ldl;
-    int rows, V, k, split;
+    int V, k, split;
     double inv_t;  // 1 / temperature
     float c;       // times log2(e)
     // Maxima m (above < m, |m| <= most) for which a tile's exponents are
@@ -625,7 +631,7 @@ int quantr_logprobs_dev(const void* x, long long ldl, uint32_t type, int rows, i
     if (!kv8_aligned({token, logprob, entropy, lse, top_id, top_logprob})) return QUANTR_ERR_BAD_ARG;
     (void)workspace, (void)workspace_bytes;
     LpArgs a{};
-    a.x = x, a.ldl = ldl, a.rows = rows, a.V = vocab, a.k = k, a.split = lp_split(rows, vocab);
+    a.x = x, a.ldl = ldl, a.V = vocab, a.k = k, a.split = lp_split(rows, vocab);
     if ((long long)rows * a.split > 0x7fffffffll) return QUANTR_ERR_TOO_LARGE;
     a.inv_t = 1.0 / (double)temperature;
     a.c = (float)(1.4426950408889634 / (double)temperature);
