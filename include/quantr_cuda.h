@@ -515,7 +515,7 @@ typedef struct {
 
 /* A ragged batch of rows (new tokens, query tokens): sequence b of B is slot
  * slot[b] (NULL: b) and has the rows start[b] .. start[b+1]-1 (NULL start:
- * max_rows rows each), at most max_rows of them.  Its rows are the LAST tokens
+ * max_rows rows each, B*max_rows < 2^31), at most max_rows of them.  Its rows are the LAST tokens
  * of the sequence: with n rows, row i stands at position lens - n + i, so lens
  * already counts them (quantr_kv8_extend_dev).  No slot appears twice. */
 typedef struct {

@@ -47,7 +47,9 @@ inline int kv8_check_tables(const quantr_kv8_tables* t)
 // A batch of no sequences or no rows is allowed (the calls do nothing).
 inline int kv8_check_batch(const quantr_kv8_batch* b)
 {
-    return b && b->B >= 0 && b->max_rows >= 0 && kv8_aligned({b->slot, b->start}) ? QUANTR_OK : QUANTR_ERR_BAD_ARG;
+    if (!b || b->B < 0 || b->max_rows < 0 || !kv8_aligned({b->slot, b->start})) return QUANTR_ERR_BAD_ARG;
+    // Row numbers are 32-bit, those that `start` gives already.
+    return b->start || (long long)b->B * b->max_rows <= 0x7fffffffll ? QUANTR_OK : QUANTR_ERR_TOO_LARGE;
 }
 
 inline size_t kv8_type_bytes(uint32_t type) { return type == QUANTR_TYPE_F32 ? 4 : 2; }
